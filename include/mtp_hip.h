@@ -576,6 +576,132 @@ int mtp_batch_prefix_match(const int64_t *ids, int64_t R, int64_t L,
                            int32_t *out, void *stream);
 
 /* ------------------------------------------------------------------------- */
+/* Serving around the paged cache (no counterparts in the reference)         */
+/* ------------------------------------------------------------------------- */
+
+/*
+ * Norms of queries and keys for each head with the position rotation in the
+ * same pass:
+ *   y = x * rsqrt(mean_d(x^2) + eps) * w     (norm = 0: y = x; weight NULL: ones)
+ *   (y_a, y_b) -> (y_a cos t - y_b sin t, y_b cos t + y_a sin t),
+ *   t = position * inv_freq[i], i < rot / 2,
+ * (a, b) = (i, i + rot / 2), or (2 i, 2 i + 1) with interleaved = 1; elements
+ * from rot on are not rotated. q [B, H, T, D], k [B, Hk, T, D] and the outputs
+ * by element strides (batch, head, token), d contiguous, all in dtype (F32,
+ * BF16, F16); D <= 4096. inv_freq [rot / 2] fp32, or fp64 with freq_f64 = 1;
+ * q_weight / k_weight [D] fp32. The position of token t of row b is
+ * positions[b * pos_sb + t] (device int64), or start + t where positions is
+ * NULL; start as in mtp_paged_kv_write. The angle is reduced in 64 bits;
+ * everything else is fp32, rounded once.
+ */
+int mtp_qk_norm_rope(const void *q, const void *k, int dtype, int64_t B,
+                     int64_t T, int64_t H, int64_t Hk, int64_t D, int64_t q_sb,
+                     int64_t q_sh, int64_t q_st, int64_t k_sb, int64_t k_sh,
+                     int64_t k_st, const void *inv_freq, int freq_f64,
+                     int64_t rot, int interleaved, int norm,
+                     const float *q_weight, const float *k_weight, float eps,
+                     const int64_t *positions, int64_t pos_sb,
+                     const int64_t *start_dev, int start_per_row,
+                     int64_t start_host, void *q_out, int64_t qo_sb,
+                     int64_t qo_sh, int64_t qo_st, void *k_out, int64_t ko_sb,
+                     int64_t ko_sh, int64_t ko_st, void *stream);
+
+/*
+ * The same, with the keys written into their pages beside the values v [B,
+ * Hk, T, D], which pass unchanged: token t of row b goes to logical position
+ * start + t, as in mtp_paged_kv_write (positions outside the table and pages
+ * outside [0, num_pages) are skipped). Pages [num_pages, B, Hk, page_size, D]
+ * in dtype; page_table [B, ld_tab] int32.
+ */
+int mtp_qk_norm_rope_write(
+    const void *q, const void *k, const void *v, int dtype, int64_t B,
+    int64_t T, int64_t H, int64_t Hk, int64_t D, int64_t q_sb, int64_t q_sh,
+    int64_t q_st, int64_t k_sb, int64_t k_sh, int64_t k_st, int64_t v_sb,
+    int64_t v_sh, int64_t v_st, const void *inv_freq, int freq_f64, int64_t rot,
+    int interleaved, int norm, const float *q_weight, const float *k_weight,
+    float eps, const int64_t *positions, int64_t pos_sb,
+    const int64_t *start_dev, int start_per_row, int64_t start_host,
+    void *q_out, int64_t qo_sb, int64_t qo_sh, int64_t qo_st, void *k_pages,
+    void *v_pages, int64_t num_pages, int64_t page_size,
+    const int32_t *page_table, int64_t ld_tab, void *stream);
+
+/*
+ * Attention of a prompt (or of a chunk behind earlier keys) with a sliding
+ * window and a few first keys that stay visible:
+ *   out[b, h, t] = softmax_j(q[b, h, t] . k[b, hk, j] * scale) @ v[b, hk, j],
+ *   hk = h / (H / Hk), over the keys j <= pos with pos - j < window or
+ *   j < sinks,  pos = L - T + t.
+ * q / out [B, H, T, D], k / v [B, Hk, L, D] by element strides (batch, head,
+ * token), d contiguous, in dtype; H a multiple of Hk, T <= L, D <= 1024.
+ * window -1: every earlier key; window >= 1 counts the query's own position.
+ * lengths NULL or device int64 [B]: keys and queries at positions >=
+ * lengths[b] are padding: such keys are never read, such rows are zero. A row
+ * that sees no key is zero.
+ */
+int mtp_window_attention(const void *q, int dtype, int64_t B, int64_t H,
+                         int64_t Hk, int64_t T, int64_t D, int64_t q_sb,
+                         int64_t q_sh, int64_t q_st, const void *k,
+                         int64_t k_sb, int64_t k_sh, int64_t k_st,
+                         const void *v, int64_t v_sb, int64_t v_sh,
+                         int64_t v_st, int64_t L, int64_t window,
+                         int64_t sinks, const int64_t *lengths, float scale,
+                         void *out, int64_t o_sb, int64_t o_sh, int64_t o_st,
+                         void *workspace, size_t workspace_bytes,
+                         void *stream);
+
+/*
+ * The same for a few new tokens whose keys are in the paged cache already:
+ * pos = start + t, start as in mtp_paged_kv_write (device int64, shared or
+ * one per row, or start_host), key j of row b in slot j % page_size of page
+ * page_table[b, j] (a page outside [0, num_pages) hides its key; keys end at
+ * the table's width L); pages [num_pages, B, Hk, page_size, D] in dtype. A
+ * negative position sees no key (a padded row of a batch: start = -T).
+ * weights NULL or fp32 [B, Hk, L]: the weight that each key received from
+ * this call's queries is added, summed over the T queries and the H / Hk
+ * heads of its key head.
+ */
+int mtp_paged_window_attention(
+    const void *q, int dtype, int64_t B, int64_t H, int64_t Hk, int64_t T,
+    int64_t D, int64_t q_sb, int64_t q_sh, int64_t q_st, const void *k_pages,
+    const void *v_pages, int64_t num_pages, const int32_t *page_table,
+    int64_t L, int64_t page_size, const int64_t *start_dev, int start_per_row,
+    int64_t start_host, int64_t window, int64_t sinks, float scale, void *out,
+    int64_t o_sb, int64_t o_sh, int64_t o_st, float *weights, void *workspace,
+    size_t workspace_bytes, void *stream);
+
+/* Workspace bytes of the two entry points above (paged = 0 / 1; weights = 1
+ * where the paged one is given weights). */
+size_t mtp_window_attention_workspace_bytes(int dtype, int64_t B, int64_t H,
+                                            int64_t Hk, int64_t T, int64_t D,
+                                            int64_t L, int64_t window,
+                                            int64_t sinks, int paged,
+                                            int weights);
+
+/*
+ * Eviction from the paged cache: of the lengths[b] entries of row b's table
+ * each key head keeps its first `sinks`, its last `recent` and, up to `keep`
+ * in all, the others of largest weight (equal weights: the lower position;
+ * NaN counts as the largest). Entries whose page is outside [0, num_pages)
+ * hold no key and are never kept. The kept rows of K and V are copied in the
+ * order of their positions to positions 0 .. of out_table [B, keep] (pages
+ * outside the pool are skipped; rows past the new length keep what they
+ * hold). No page of out_table may hold an entry of row b's page_table.
+ *   kept [B, Hk, keep] int32: the positions, -1 past the new length
+ *   out_weights [B, Hk, keep] fp32: their weights, 0 past it
+ *   out_lengths [B] int64: entries kept
+ * weights [B, Hk, L] fp32, lengths [B] int64, page_table [B, L] int32; pages
+ * [num_pages, B, Hk, page_size, row_bytes]; sinks + recent <= keep. Two
+ * launches, no workspace.
+ */
+int mtp_kv_evict(const float *weights, const int64_t *lengths, int64_t B,
+                 int64_t Hk, int64_t L, int64_t keep, int64_t sinks,
+                 int64_t recent, void *k_pages, void *v_pages,
+                 int64_t num_pages, int64_t page_size, int64_t row_bytes,
+                 const int32_t *page_table, const int32_t *out_table,
+                 int32_t *kept, float *out_weights, int64_t *out_lengths,
+                 void *stream);
+
+/* ------------------------------------------------------------------------- */
 /* Workspace                                                                 */
 /* ------------------------------------------------------------------------- */
 

@@ -29,31 +29,6 @@
 
 namespace mtp {
 
-// x + the value of the lane that the DPP control selects
-template <int CTRL>
-__device__ __forceinline__ float dpp_add(float x) {
-  return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
-}
-// Sum over aligned groups of N lanes, in every lane of the group.
-template <int N>
-__device__ __forceinline__ float sum_over_lanes(float x) {
-  if constexpr (N >= 2) x = dpp_add<0xB1>(x);    // quad_perm 1 0 3 2
-  if constexpr (N >= 4) x = dpp_add<0x4E>(x);    // quad_perm 2 3 0 1
-  if constexpr (N >= 8) x = dpp_add<0x141>(x);   // row_half_mirror
-  if constexpr (N >= 16) x = dpp_add<0x140>(x);  // row_mirror
-  if constexpr (N >= 32) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false,
-                                                    false);
-    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-  }
-  if constexpr (N >= 64) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
-                                                    false);
-    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-  }
-  return x;
-}
-
 // 16 bytes of a row of element type KT as fp32.
 template <int KT>
 __device__ __forceinline__ void dec_unpack(u32x4 w, float *f) {

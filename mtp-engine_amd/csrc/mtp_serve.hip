@@ -1,0 +1,381 @@
+// C ABI of the serving operators around the paged KV cache: per-head norms
+// with the position rotation, windowed attention of prompts and of new tokens
+// over the cache, eviction by attention weight. Declarations are in
+// include/mtp_hip.h.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "abi_util.hpp"
+#include "evict.hpp"
+#include "rope.hpp"
+#include "wattn.hpp"
+
+using namespace mtp;
+
+namespace {
+
+bool mult(std::initializer_list<int64_t> v, int64_t m) {
+  for (int64_t x : v)
+    if (x % m != 0) return false;
+  return true;
+}
+
+// ---- norms and rotation
+typedef void (*RopeKernel)(RopeArgs);
+
+template <int DT, int LPR>
+RopeKernel rope_form(bool inter) {
+  return inter ? rope_kernel<DT, LPR, true> : rope_kernel<DT, LPR, false>;
+}
+template <int DT>
+RopeKernel rope_lanes(int64_t chunks, bool inter, int &lpr) {
+  if (chunks <= 4) return lpr = 4, rope_form<DT, 4>(inter);
+  if (chunks <= 8) return lpr = 8, rope_form<DT, 8>(inter);
+  if (chunks <= 16) return lpr = 16, rope_form<DT, 16>(inter);
+  if (chunks <= 32) return lpr = 32, rope_form<DT, 32>(inter);
+  if (chunks <= 64) return lpr = 64, rope_form<DT, 64>(inter);
+  return nullptr;
+}
+
+// The 16-byte form, or null: rows, strides and addresses of whole 16 bytes,
+// a rotation whose halves are whole chunks.
+RopeKernel rope_pick(const RopeArgs &a, int dt, int &lpr) {
+  const int64_t e = 16 / dtype_bytes(dt);
+  if (a.D % e != 0 || (a.interleaved ? a.rot % e : (a.rot / 2) % e) != 0) return nullptr;
+  if (!aligned16(a.q) || !aligned16(a.k) || !aligned16(a.qo) || (a.ko && !aligned16(a.ko)) ||
+      (a.v && (!aligned16(a.v) || !aligned16(a.k_pages) || !aligned16(a.v_pages))))
+    return nullptr;
+  if (!mult({a.q_sb, a.q_sh, a.q_st, a.k_sb, a.k_sh, a.k_st, a.v_sb, a.v_sh, a.v_st, a.qo_sb,
+             a.qo_sh, a.qo_st, a.ko_sb, a.ko_sh, a.ko_st},
+            e))
+    return nullptr;
+  switch (dt) {
+    case MTP_F32: return rope_lanes<MTP_F32>(a.D / e, a.interleaved, lpr);
+    case MTP_BF16: return rope_lanes<MTP_BF16>(a.D / e, a.interleaved, lpr);
+    case MTP_F16: return rope_lanes<MTP_F16>(a.D / e, a.interleaved, lpr);
+  }
+  return nullptr;
+}
+
+int rope_launch(RopeArgs &a, int dt, hipStream_t st) {
+  int lpr = 0;
+  const int64_t toks = (int64_t)a.B * a.T;
+  const int64_t nr = a.H + a.Hk + (a.v ? a.Hk : 0);
+  if (RopeKernel k = rope_pick(a, dt, lpr)) {
+    // a wave per token, more of them while the chip has room
+    const int64_t rpi = 64 / lpr, room = (int64_t)device_cus() * 8;
+    a.hs = (int)std::max<int64_t>(1, std::min((room + toks - 1) / toks, (nr + rpi - 1) / rpi));
+    const int64_t blocks = (toks * a.hs + 3) / 4;
+    if (blocks > INT32_MAX) return MTP_ERR_SHAPE;
+    hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(256), 0, st, a);
+  } else {
+    if (toks * nr > INT32_MAX) return MTP_ERR_SHAPE;
+    hipLaunchKernelGGL(rope_generic_kernel, dim3((unsigned)(toks * nr)), dim3(64), 0, st, a, dt);
+  }
+  return launch_status();
+}
+
+// What both entry points check and fill in; > 0: nothing to do.
+int rope_args(RopeArgs &a, const void *q, const void *k, int dtype, int64_t B, int64_t T, int64_t H,
+              int64_t Hk, int64_t D, const void *inv_freq, int freq_f64, int64_t rot,
+              int interleaved, int norm, const float *q_weight, const float *k_weight, float eps,
+              const int64_t *positions, int64_t pos_sb, const int64_t *start_dev,
+              int start_per_row, int64_t start_host, void *q_out) {
+  if (!is_float_dt(dtype)) return MTP_ERR_DTYPE;
+  if (B < 0 || T < 0 || H < 0 || Hk < 0 || D <= 0 || D > kRopeMaxD || rot < 0 || rot > D ||
+      rot % 2 != 0 || B > INT32_MAX || T > INT32_MAX || H > 65535 || Hk > 65535)
+    return MTP_ERR_SHAPE;
+  if (B == 0 || T == 0 || H + Hk == 0) return 1;
+  if ((H > 0 && (!q || !q_out)) || (Hk > 0 && !k) || (rot > 0 && !inv_freq)) return MTP_ERR_NULL;
+  a.q = q;
+  a.k = k;
+  a.qo = q_out;
+  a.inv_freq = inv_freq;
+  a.freq64 = freq_f64 ? 1 : 0;
+  a.wq = q_weight;
+  a.wk = k_weight;
+  a.pos = positions;
+  a.pos_sb = pos_sb;
+  a.start_dev = start_dev;
+  a.start_per_row = start_per_row ? 1 : 0;
+  a.start_host = start_host;
+  a.B = (int)B;
+  a.T = (int)T;
+  a.H = (int)H;
+  a.Hk = (int)Hk;
+  a.D = (int)D;
+  a.rot = (int)rot;
+  a.norm = norm ? 1 : 0;
+  a.interleaved = interleaved ? 1 : 0;
+  a.eps = eps;
+  return MTP_OK;
+}
+
+// ---- windowed attention
+struct WinPlan {
+  int64_t ld_sc = 0;
+  size_t ml_off = 0, total = 0;
+};
+
+// Keys that T queries can see of a sequence at most.
+int64_t win_most(int64_t T, int64_t L, int64_t window, int64_t sinks) {
+  if (window < 0 || window >= kWinNone / 2) return L;
+  return std::min(L, std::min(sinks, L) + window + T - 1);
+}
+
+WinPlan win_plan(int64_t B, int64_t H, int64_t Hk, int64_t T, int64_t L, int64_t window,
+                 int64_t sinks, bool weights) {
+  WinPlan p;
+  if (B <= 0 || H <= 0 || Hk <= 0 || T <= 0 || L <= 0) return p;
+  if (weights) {
+    p.ld_sc = win_most(T, L, window, sinks);
+    p.ml_off = kCounterBytes + align_up((size_t)(B * H * T) * (size_t)p.ld_sc * 4, 256);
+    p.total = p.ml_off + align_up((size_t)(B * H * T) * 8, 256);
+  }
+  return p;
+}
+
+template <bool PAGED>
+void (*win_generic(int64_t d))(WinArgs, int) {
+  if (d <= 64) return win_rows_generic_kernel<1, PAGED>;
+  if (d <= 128) return win_rows_generic_kernel<2, PAGED>;
+  if (d <= 256) return win_rows_generic_kernel<4, PAGED>;
+  return win_rows_generic_kernel<16, PAGED>;
+}
+constexpr int64_t kWinMaxD = 1024;
+
+int win_launch(WinArgs &a, int dt, void *workspace, size_t workspace_bytes, hipStream_t st) {
+  const WinPlan p = win_plan(a.B, a.H, a.Hk, a.T, a.L, a.window == kWinNone ? -1 : a.window,
+                             a.sinks, a.weights != nullptr);
+  if (p.total > 0 && (!workspace || workspace_bytes < p.total)) return MTP_ERR_WORKSPACE;
+  unsigned char *const w8 = (unsigned char *)workspace;
+  if (a.weights) {
+    a.scores = (float *)(w8 + kCounterBytes);
+    a.ld_sc = p.ld_sc;
+    a.ml = (float *)(w8 + p.ml_off);
+  }
+  const int64_t rows = (int64_t)a.B * a.H * a.T;
+  if (rows > INT32_MAX) return MTP_ERR_SHAPE;
+  hipLaunchKernelGGL(a.table ? win_generic<true>(a.D) : win_generic<false>(a.D),
+                     dim3((unsigned)rows), dim3(64), win_row_lds(a.D) * 4, st, a, dt);
+  const int s = launch_status();
+  if (s != MTP_OK || !a.weights) return s;
+  if ((int64_t)a.B * a.Hk > 65535) return MTP_ERR_SHAPE;
+  hipLaunchKernelGGL(win_weights_kernel, dim3((unsigned)((p.ld_sc + 255) / 256),
+                                              (unsigned)(a.B * a.Hk)),
+                     dim3(256), 0, st, a);
+  return launch_status();
+}
+
+// What both entry points check and fill in; > 0: nothing to do.
+int win_args(WinArgs &a, const void *q, int dtype, int64_t B, int64_t H, int64_t Hk, int64_t T,
+             int64_t D, int64_t q_sb, int64_t q_sh, int64_t q_st, const void *k, const void *v,
+             int64_t L, int64_t window, int64_t sinks, float scale, void *out, int64_t o_sb,
+             int64_t o_sh, int64_t o_st) {
+  if (!is_float_dt(dtype)) return MTP_ERR_DTYPE;
+  if (B < 0 || T < 0 || H < 0 || Hk <= 0 || H % Hk != 0 || D <= 0 || D > kWinMaxD || L < 0 ||
+      B > INT32_MAX || H > 65535 || T > kWinMaxKeys || L > kWinMaxKeys)
+    return MTP_ERR_SHAPE;
+  if (window == 0 || window < -1 || sinks < 0) return MTP_ERR_ARG;
+  if (B == 0 || T == 0 || H == 0) return 1;
+  if (!q || !out || (L > 0 && (!k || !v))) return MTP_ERR_NULL;
+  a.q = q;
+  a.q_sb = q_sb;
+  a.q_sh = q_sh;
+  a.q_st = q_st;
+  a.k = k;
+  a.v = v;
+  a.out = out;
+  a.o_sb = o_sb;
+  a.o_sh = o_sh;
+  a.o_st = o_st;
+  a.B = (int)B;
+  a.H = (int)H;
+  a.Hk = (int)Hk;
+  a.G = (int)(H / Hk);
+  a.T = (int)T;
+  a.D = (int)D;
+  a.L = (int)L;
+  a.window = window < 0 || window >= kWinNone / 2 ? kWinNone : (int)window;
+  a.sinks = (int)std::min(sinks, L);
+  a.scale = scale * 1.44269504088896340736f;
+  a.nchunks = 1;
+  return MTP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mtp_qk_norm_rope(const void *q, const void *k, int dtype, int64_t B, int64_t T, int64_t H,
+                     int64_t Hk, int64_t D, int64_t q_sb, int64_t q_sh, int64_t q_st, int64_t k_sb,
+                     int64_t k_sh, int64_t k_st, const void *inv_freq, int freq_f64, int64_t rot,
+                     int interleaved, int norm, const float *q_weight, const float *k_weight,
+                     float eps, const int64_t *positions, int64_t pos_sb, const int64_t *start_dev,
+                     int start_per_row, int64_t start_host, void *q_out, int64_t qo_sb,
+                     int64_t qo_sh, int64_t qo_st, void *k_out, int64_t ko_sb, int64_t ko_sh,
+                     int64_t ko_st, void *stream) {
+  RopeArgs a{};
+  const int s = rope_args(a, q, k, dtype, B, T, H, Hk, D, inv_freq, freq_f64, rot, interleaved,
+                          norm, q_weight, k_weight, eps, positions, pos_sb, start_dev,
+                          start_per_row, start_host, q_out);
+  if (s != MTP_OK) return s > 0 ? MTP_OK : s;
+  if (Hk > 0 && !k_out) return MTP_ERR_NULL;
+  a.q_sb = q_sb, a.q_sh = q_sh, a.q_st = q_st;
+  a.k_sb = k_sb, a.k_sh = k_sh, a.k_st = k_st;
+  a.qo_sb = qo_sb, a.qo_sh = qo_sh, a.qo_st = qo_st;
+  a.ko = k_out;
+  a.ko_sb = ko_sb, a.ko_sh = ko_sh, a.ko_st = ko_st;
+  return rope_launch(a, dtype, (hipStream_t)stream);
+}
+
+int mtp_qk_norm_rope_write(const void *q, const void *k, const void *v, int dtype, int64_t B,
+                           int64_t T, int64_t H, int64_t Hk, int64_t D, int64_t q_sb, int64_t q_sh,
+                           int64_t q_st, int64_t k_sb, int64_t k_sh, int64_t k_st, int64_t v_sb,
+                           int64_t v_sh, int64_t v_st, const void *inv_freq, int freq_f64,
+                           int64_t rot, int interleaved, int norm, const float *q_weight,
+                           const float *k_weight, float eps, const int64_t *positions,
+                           int64_t pos_sb, const int64_t *start_dev, int start_per_row,
+                           int64_t start_host, void *q_out, int64_t qo_sb, int64_t qo_sh,
+                           int64_t qo_st, void *k_pages, void *v_pages, int64_t num_pages,
+                           int64_t page_size, const int32_t *page_table, int64_t ld_tab,
+                           void *stream) {
+  RopeArgs a{};
+  const int s = rope_args(a, q, k, dtype, B, T, H, Hk, D, inv_freq, freq_f64, rot, interleaved,
+                          norm, q_weight, k_weight, eps, positions, pos_sb, start_dev,
+                          start_per_row, start_host, q_out);
+  if (s < 0) return s;
+  if (num_pages < 0 || page_size <= 0 || ld_tab < 0 || num_pages > INT32_MAX ||
+      page_size > INT32_MAX)
+    return MTP_ERR_SHAPE;
+  if (s > 0) return MTP_OK;
+  if (Hk > 0 && (!v || !k_pages || !v_pages || (ld_tab > 0 && !page_table))) return MTP_ERR_NULL;
+  a.q_sb = q_sb, a.q_sh = q_sh, a.q_st = q_st;
+  a.k_sb = k_sb, a.k_sh = k_sh, a.k_st = k_st;
+  a.v = v;
+  a.v_sb = v_sb, a.v_sh = v_sh, a.v_st = v_st;
+  a.qo_sb = qo_sb, a.qo_sh = qo_sh, a.qo_st = qo_st;
+  a.k_pages = k_pages;
+  a.v_pages = v_pages;
+  a.p_sh = page_size * D;
+  a.p_sb = Hk * a.p_sh;
+  a.p_sp = B * a.p_sb;
+  a.table = page_table;
+  a.ld_tab = ld_tab;
+  a.page_size = (int)page_size;
+  a.npages = (int)num_pages;
+  return rope_launch(a, dtype, (hipStream_t)stream);
+}
+
+size_t mtp_window_attention_workspace_bytes(int dtype, int64_t B, int64_t H, int64_t Hk, int64_t T,
+                                            int64_t D, int64_t L, int64_t window, int64_t sinks,
+                                            int paged, int weights) {
+  (void)dtype, (void)D, (void)paged;
+  return win_plan(B, H, Hk, T, L, window, sinks, weights != 0).total;
+}
+
+int mtp_window_attention(const void *q, int dtype, int64_t B, int64_t H, int64_t Hk, int64_t T,
+                         int64_t D, int64_t q_sb, int64_t q_sh, int64_t q_st, const void *k,
+                         int64_t k_sb, int64_t k_sh, int64_t k_st, const void *v, int64_t v_sb,
+                         int64_t v_sh, int64_t v_st, int64_t L, int64_t window, int64_t sinks,
+                         const int64_t *lengths, float scale, void *out, int64_t o_sb,
+                         int64_t o_sh, int64_t o_st, void *workspace, size_t workspace_bytes,
+                         void *stream) {
+  WinArgs a{};
+  const int s = win_args(a, q, dtype, B, H, Hk, T, D, q_sb, q_sh, q_st, k, v, L, window, sinks,
+                         scale, out, o_sb, o_sh, o_st);
+  if (s < 0) return s;
+  if (L < T) return MTP_ERR_SHAPE;
+  if (s > 0) return MTP_OK;
+  a.k_sb = k_sb, a.k_sh = k_sh, a.k_st = k_st;
+  a.v_sb = v_sb, a.v_sh = v_sh, a.v_st = v_st;
+  a.start_host = L - T;
+  a.lengths = lengths;
+  return win_launch(a, dtype, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+int mtp_paged_window_attention(const void *q, int dtype, int64_t B, int64_t H, int64_t Hk,
+                               int64_t T, int64_t D, int64_t q_sb, int64_t q_sh, int64_t q_st,
+                               const void *k_pages, const void *v_pages, int64_t num_pages,
+                               const int32_t *page_table, int64_t L, int64_t page_size,
+                               const int64_t *start_dev, int start_per_row, int64_t start_host,
+                               int64_t window, int64_t sinks, float scale, void *out, int64_t o_sb,
+                               int64_t o_sh, int64_t o_st, float *weights, void *workspace,
+                               size_t workspace_bytes, void *stream) {
+  WinArgs a{};
+  const int s = win_args(a, q, dtype, B, H, Hk, T, D, q_sb, q_sh, q_st, k_pages, v_pages, L,
+                         window, sinks, scale, out, o_sb, o_sh, o_st);
+  if (s < 0) return s;
+  if (num_pages < 0 || num_pages > INT32_MAX || page_size <= 0 || page_size > INT32_MAX ||
+      (weights && B * Hk > 65535))
+    return MTP_ERR_SHAPE;
+  if (s > 0) return MTP_OK;
+  if (L > 0 && !page_table) return MTP_ERR_NULL;
+  a.k_st = D;
+  a.k_sh = page_size * D;
+  a.k_sb = Hk * a.k_sh;
+  a.p_sp = B * a.k_sb;
+  a.v_sb = a.k_sb, a.v_sh = a.k_sh, a.v_st = a.k_st;
+  a.table = page_table;
+  a.ld_tab = L;
+  a.page_size = (int)page_size;
+  a.npages = (int)num_pages;
+  a.start_dev = start_dev;
+  a.start_per_row = start_per_row ? 1 : 0;
+  a.start_host = start_host;
+  a.weights = L > 0 ? weights : nullptr;
+  return win_launch(a, dtype, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+int mtp_kv_evict(const float *weights, const int64_t *lengths, int64_t B, int64_t Hk, int64_t L,
+                 int64_t keep, int64_t sinks, int64_t recent, void *k_pages, void *v_pages,
+                 int64_t num_pages, int64_t page_size, int64_t row_bytes, const int32_t *page_table, const int32_t *out_table,
+                 int32_t *kept, float *out_weights, int64_t *out_lengths, void *stream) {
+  if (B < 0 || Hk < 0 || L < 0 || keep <= 0 || row_bytes <= 0 || num_pages < 0 ||
+      page_size <= 0 || num_pages > INT32_MAX || page_size > INT32_MAX || L > kWinMaxKeys ||
+      keep > kWinMaxKeys || B * Hk > INT32_MAX || row_bytes > (1 << 20))
+    return MTP_ERR_SHAPE;
+  if (sinks < 0 || recent < 0 || sinks + recent > keep) return MTP_ERR_ARG;
+  if (B == 0 || Hk == 0) return MTP_OK;
+  if (!lengths || !kept || !out_weights || !out_lengths || !out_table ||
+      (L > 0 && (!weights || !page_table)) ||
+      (num_pages > 0 && (!k_pages || !v_pages)))
+    return MTP_ERR_NULL;
+  EvictArgs a{};
+  a.weights = weights;
+  a.lengths = lengths;
+  a.table = page_table;
+  a.out_table = out_table;
+  a.B = (int)B;
+  a.Hk = (int)Hk;
+  a.L = (int)L;
+  a.keep = (int)keep;
+  a.sinks = (int)sinks;
+  a.recent = (int)recent;
+  a.npages = (int)num_pages;
+  a.page_size = (int)page_size;
+  a.k_pages = k_pages;
+  a.v_pages = v_pages;
+  a.row_bytes = row_bytes;
+  a.kept = kept;
+  a.out_weights = out_weights;
+  a.out_lengths = out_lengths;
+  hipStream_t st = (hipStream_t)stream;
+  // the copy's unit: the largest that divides a row and the addresses
+  const uintptr_t bits = (uintptr_t)row_bytes | (uintptr_t)k_pages | (uintptr_t)v_pages;
+  const int unit = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : bits % 2 == 0 ? 2 : 1;
+  const int64_t blocks = (B * Hk * keep * (row_bytes / unit) + 255) / 256;
+  if (blocks > INT32_MAX) return MTP_ERR_SHAPE;
+  hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)(B * Hk)), dim3(kEvictThreads), 0, st, a);
+  int s = launch_status();
+  if (s != MTP_OK || num_pages == 0) return s;
+  void (*const mv)(EvictArgs) = unit == 16  ? evict_move_kernel<u32x4>
+                                : unit == 4 ? evict_move_kernel<uint32_t>
+                                : unit == 2 ? evict_move_kernel<uint16_t>
+                                            : evict_move_kernel<uint8_t>;
+  hipLaunchKernelGGL(mv, dim3((unsigned)blocks), dim3(256), 0, st, a);
+  return launch_status();
+}
+
+}  // extern "C"

@@ -1,0 +1,54 @@
+// Arguments of the windowed attention kernels (wattn*.hpp), shared with the
+// host code that plans them.
+#pragma once
+
+#include <stdint.h>
+
+#include "../../include/mtp_hip.h"
+
+namespace mtp {
+
+// Key and row positions, with the window added, stay within 31 bits.
+constexpr int64_t kWinMaxKeys = (int64_t)1 << 29;
+constexpr int kWinNone = 1 << 30;  // window: every earlier key is visible
+
+struct WinArgs {
+  const void *q;                  // [B, H, T, D] by element strides, d contiguous
+  int64_t q_sb, q_sh, q_st;
+  const void *k, *v;              // dense [B, Hk, L, D] by element strides, or
+                                  // (table) pages [P, B, Hk, page_size, D]
+  int64_t k_sb, k_sh, k_st, v_sb, v_sh, v_st;
+  const int32_t *table;           // [B, ld_tab] physical page of each key, or null: dense
+  int64_t ld_tab, p_sp;           // pages: p_sp the page stride; k_sb, k_sh, k_st their others
+  int page_size, npages;
+  void *out;                      // by element strides
+  int64_t o_sb, o_sh, o_st;
+  int B, H, Hk, G, T, D;          // G = H / Hk query heads to a key head
+  int L;                          // keys of a sequence at most
+  int window, sinks;              // window: kWinNone for none
+  const int64_t *start_dev;       // position of query 0, per sequence (start_per_row) or shared
+  int start_per_row;
+  int64_t start_host;
+  const int64_t *lengths;         // [B] keys and queries of each sequence (dense), or null
+  float scale;                    // of the scores, in units of log 2
+  float *scores;                  // [B * Hk][G * T][ld_sc] masked scores, or null
+  float *ml;                      // [B * Hk][G * T][2]: maximum and sum of a row, with scores
+  int64_t ld_sc;
+  float *weights;                 // [B, Hk, L], added to
+  int nchunks;                    // key chunks of a (batch, key head, row block)
+  float *part;                    // [unit][chunk][rows][D + 2] partials, nchunks > 1
+  unsigned *ticket;               // arrivals per unit
+};
+
+// The keys that the queries of one sequence see: [0, ns) and [lo, hi), the
+// union over its rows; row t stands at position first + t and sees those keys
+// j <= first + t with j > first + t - window or j < sinks; rows from `rows` on
+// see nothing.
+struct WinSpan {
+  int first, rows, ns, lo, hi;
+  __host__ __device__ int count() const { return ns + hi - lo; }
+  // Key of compact index i < count().
+  __host__ __device__ int key(int i) const { return i < ns ? i : lo + (i - ns); }
+};
+
+}  // namespace mtp

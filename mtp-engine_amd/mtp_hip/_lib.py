@@ -94,6 +94,21 @@ SIGNATURES = {
     "mtp_verify_commit": (
         _i, [_vp, _vp, _vp, _vp, _i, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp]),
     "mtp_batch_prefix_match": (_i, [_vp, _i64, _i64, _vp, _vp]),
+    "mtp_qk_norm_rope": (
+        _i, [_vp, _vp, _i] + [_i64] * 11 + [_vp, _i, _i64, _i, _i, _vp, _vp, _f, _vp, _i64, _vp, _i,
+             _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp]),
+    "mtp_qk_norm_rope_write": (
+        _i, [_vp, _vp, _vp, _i] + [_i64] * 14 + [_vp, _i, _i64, _i, _i, _vp, _vp, _f, _vp, _i64,
+             _vp, _i, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _vp]),
+    "mtp_window_attention": (
+        _i, [_vp, _i] + [_i64] * 8 + [_vp, _i64, _i64, _i64, _vp] + [_i64] * 6 +
+        [_vp, _f, _vp, _i64, _i64, _i64, _vp, _sz, _vp]),
+    "mtp_paged_window_attention": (
+        _i, [_vp, _i] + [_i64] * 8 + [_vp, _vp, _i64, _vp, _i64, _i64, _vp, _i, _i64, _i64, _i64,
+             _f, _vp, _i64, _i64, _i64, _vp, _vp, _sz, _vp]),
+    "mtp_window_attention_workspace_bytes": (_sz, [_i] + [_i64] * 8 + [_i, _i]),
+    "mtp_kv_evict": (
+        _i, [_vp, _vp] + [_i64] * 6 + [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
     "mtp_workspace_init": (_i, [_vp, _sz, _vp]),
     "mtp_fused_multi_verify_noalloc": (
         _i, [_vp, _i, _i64, _i64, _i64, _vp, _i, _i64, _vp, _i, _vp, _i64, _vp, _vp, _vp, _vp,

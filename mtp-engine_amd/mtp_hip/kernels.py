@@ -220,6 +220,66 @@ def tree_verify_attention(
                                      v_tree, tree_mask, scale)
 
 
+def fused_qk_norm_rope(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor, start=0,
+                       positions: Optional[torch.Tensor] = None,
+                       q_weight: Optional[torch.Tensor] = None,
+                       k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                       norm: bool = True,
+                       interleaved: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Extension: RMSNorm of every query and key head with the position
+    rotation in the same pass (ops.qk_norm_rope): q [B, H, T, D], k [B, Hk, T,
+    D] at positions [T] / [B, T] or start + t. Returns (q, k)."""
+    return ops.qk_norm_rope(q, k, inv_freq, start, positions, q_weight, k_weight, eps, norm,
+                            interleaved)
+
+
+def fused_qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                             inv_freq: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                             page_table: torch.Tensor, start,
+                             positions: Optional[torch.Tensor] = None,
+                             q_weight: Optional[torch.Tensor] = None,
+                             k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                             norm: bool = True, interleaved: bool = False) -> torch.Tensor:
+    """Extension: fused_qk_norm_rope with the keys and the values v written
+    into the pages of the positions start + t (ops.qk_norm_rope_write).
+    Returns the queries."""
+    return ops.qk_norm_rope_write(q, k, v, inv_freq, k_pages, v_pages, page_table, start,
+                                  positions, q_weight, k_weight, eps, norm, interleaved)
+
+
+def fused_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                           window: Optional[int] = None, sinks: int = 0,
+                           lengths: Optional[torch.Tensor] = None,
+                           scale: Optional[float] = None) -> torch.Tensor:
+    """Extension: causal attention of a prompt (or of a chunk behind earlier
+    keys) with a sliding window and `sinks` first keys that stay visible
+    (ops.window_attention): q [B, H, T, D]; k / v [B, Hk, L, D]; lengths [B]
+    of a padded batch."""
+    return ops.window_attention(q, k, v, window, sinks, lengths, scale)
+
+
+def fused_paged_window_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                                 page_table: torch.Tensor, page_size: int, start,
+                                 window: Optional[int] = None, sinks: int = 0,
+                                 scale: Optional[float] = None,
+                                 weights: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Extension: fused_window_attention of the T newest tokens over a paged
+    cache (ops.paged_window_attention): q [B, H, T, D] at positions start + t;
+    weights [B, Hk, L] takes the weight that each key received."""
+    return ops.paged_window_attention(q, k_pages, v_pages, page_table, page_size, start, window,
+                                      sinks, scale, weights)
+
+
+def kv_evict(weights: torch.Tensor, lengths: torch.Tensor, k_pages: torch.Tensor,
+             v_pages: torch.Tensor, page_table: torch.Tensor, out_table: torch.Tensor,
+             sinks: int = 0,
+             recent: int = 0) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Extension: cut a paged cache to out_table.shape[1] entries per key head
+    by the weight its keys received (ops.kv_evict). Returns (kept positions,
+    their weights, new lengths)."""
+    return ops.kv_evict(weights, lengths, k_pages, v_pages, page_table, out_table, sinks, recent)
+
+
 def quantize_fp8_e4m3(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """(x_fp8, scale) with scale = amax(|x|) / 448 (1 when amax is not > 0)
     (mtp_kernels.py:704-713)."""

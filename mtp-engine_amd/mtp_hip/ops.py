@@ -8,6 +8,7 @@ synchronising. Inputs must live on a HIP device.
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional, Tuple
 
@@ -680,3 +681,289 @@ def batch_prefix_match(ids: torch.Tensor) -> torch.Tensor:
     s = lib.mtp_batch_prefix_match(ptr(ids), R, L, ptr(out), _lib.stream_handle(ids.device))
     check(s, "batch_prefix_match")
     return out
+
+
+# ---------------------------------------------------------------------------
+# Serving around the paged cache
+def _on_its_device(fn):
+    """The call runs with its first tensor's device as the current one: a
+    launch goes to the current device whatever its stream."""
+    @functools.wraps(fn)
+    def call(first, *args, **kwargs):
+        if first.is_cuda and first.get_device() != torch.cuda.current_device():
+            with torch.cuda.device(first.device):
+                return fn(first, *args, **kwargs)
+        return fn(first, *args, **kwargs)
+    return call
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    return t if t.stride(-1) == 1 else t.contiguous()
+
+
+def _start_arg(name: str, start, B: int):
+    """(device tensor or None, per row, host value) of a start position: an
+    int, or an int64 device tensor of one element (shared) or [B]."""
+    if torch.is_tensor(start):
+        dev = start.contiguous().to(torch.int64)
+        assert dev.numel() in (1, B), f"{name}: start must hold 1 or B positions"
+        return dev, int(dev.numel() == B and B > 1), 0
+    return None, 0, int(start)
+
+
+def _pages_arg(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+               B: int, Hk: int, D: int, dtype) -> torch.Tensor:
+    """Checks pages [P, B, Hk, page_size, D] and the table [B, L]; the table
+    as int32."""
+    assert k_pages.dim() == 5 and k_pages.is_contiguous() and v_pages.is_contiguous() and \
+        v_pages.shape == k_pages.shape, \
+        f"{name}: pages must be contiguous [P, B, Hk, page_size, D], both alike"
+    assert (k_pages.shape[1], k_pages.shape[2], k_pages.shape[4]) == (B, Hk, D), \
+        f"{name}: pages {tuple(k_pages.shape)} do not match B={B}, Hk={Hk}, D={D}"
+    assert k_pages.dtype == dtype and v_pages.dtype == dtype, f"{name}: dtypes differ"
+    assert page_table.dim() == 2 and page_table.shape[0] == B, f"{name}: page_table [{B}, L]"
+    return _i32(page_table.contiguous())
+
+
+def _rope_args(name: str, q, k, inv_freq, start, positions, q_weight, k_weight):
+    assert q.dim() == 4 and k.dim() == 4, f"{name}: q [B, H, T, D], k [B, Hk, T, D]"
+    q, k = _rows(q), _rows(k)
+    B, H, T, D = q.shape
+    assert (k.shape[0], k.shape[2], k.shape[3]) == (B, T, D), \
+        f"{name}: k must be [{B}, Hk, {T}, {D}], got {tuple(k.shape)}"
+    assert k.dtype == q.dtype, f"{name}: dtypes differ"
+    inv_freq = inv_freq.contiguous()
+    if inv_freq.dtype not in (torch.float32, torch.float64):
+        raise TypeError(f"{name}: inv_freq must be float32 or float64, got {inv_freq.dtype}")
+    rot = 2 * inv_freq.numel()
+    assert inv_freq.dim() == 1 and rot <= D, f"{name}: inv_freq holds at most D / 2 frequencies"
+    pos_sb = 0
+    if positions is not None:
+        assert positions.dim() in (1, 2) and positions.shape[-1] == T and \
+            (positions.dim() == 1 or positions.shape[0] in (1, B)), \
+            f"{name}: positions must be [{T}], [1, {T}] or [{B}, {T}]"
+        positions = positions.contiguous().to(torch.int64)
+        pos_sb = T if positions.dim() == 2 and positions.shape[0] == B else 0
+    ws = []
+    for w in (q_weight, k_weight):
+        if w is not None:
+            w = _f32(w.contiguous())
+            assert w.numel() == D, f"{name}: a norm weight has {w.numel()} != {D}"
+        ws.append(w)
+    start_dev, per_row, start_host = _start_arg(name, start, B)
+    return q, k, inv_freq, rot, positions, pos_sb, ws[0], ws[1], start_dev, per_row, start_host
+
+
+@_on_its_device
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor, start=0,
+                 positions: Optional[torch.Tensor] = None,
+                 q_weight: Optional[torch.Tensor] = None,
+                 k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, norm: bool = True,
+                 interleaved: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(q, k) with every head's row normed (x * rsqrt(mean(x^2) + eps) *
+    weight; norm=False: as it is) and its first 2 * len(inv_freq) elements
+    rotated by position * inv_freq: pairs (i, i + half), interleaved=True
+    (2 i, 2 i + 1). q [B, H, T, D], k [B, Hk, T, D] (any strides with d
+    contiguous, e.g. slices of one projection); weights [D]; token t stands at
+    positions [T] or [B, T] (int64) or, without, at start + t, start as in
+    paged_kv_write. The outputs keep the inputs' order of dimensions in
+    memory."""
+    name = "qk_norm_rope"
+    lib = _lib.load()
+    q, k, f, rot, positions, pos_sb, wq, wk, start_dev, per_row, start_host = _rope_args(
+        name, q, k, inv_freq, start, positions, q_weight, k_weight)
+    _on_device("q", q, k=k, inv_freq=f, positions=positions, q_weight=wq, k_weight=wk,
+               start=start_dev)
+    B, H, T, D = q.shape
+    qo, ko = torch.empty_like(q), torch.empty_like(k)
+    s = lib.mtp_qk_norm_rope(
+        ptr(q), ptr(k), code(q.dtype), B, T, H, k.shape[1], D, *q.stride()[:3], *k.stride()[:3],
+        ptr(f), int(f.dtype is torch.float64), rot, int(bool(interleaved)), int(bool(norm)),
+        ptr(wq), ptr(wk), float(eps), ptr(positions), pos_sb, ptr(start_dev), per_row, start_host,
+        ptr(qo), *qo.stride()[:3], ptr(ko), *ko.stride()[:3], _lib.stream_handle(q.device))
+    check(s, name)
+    return qo, ko
+
+
+@_on_its_device
+def qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, inv_freq: torch.Tensor,
+                       k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                       start, positions: Optional[torch.Tensor] = None,
+                       q_weight: Optional[torch.Tensor] = None,
+                       k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                       norm: bool = True, interleaved: bool = False) -> torch.Tensor:
+    """qk_norm_rope and paged_kv_write in one launch: returns the queries and
+    writes the normed, rotated keys and the values v [B, Hk, T, D] into the
+    pages of the positions start + t (which `positions`, the angles, need not
+    equal: the nodes of a draft tree stand at their depth). Pages [P, B, Hk,
+    page_size, D] in q's dtype; positions outside the table and pages outside
+    the pool are skipped."""
+    name = "qk_norm_rope_write"
+    lib = _lib.load()
+    q, k, f, rot, positions, pos_sb, wq, wk, start_dev, per_row, start_host = _rope_args(
+        name, q, k, inv_freq, start, positions, q_weight, k_weight)
+    v = _rows(v)
+    assert v.shape == k.shape, f"{name}: v must be shaped like k, got {tuple(v.shape)}"
+    assert v.dtype == q.dtype, f"{name}: dtypes differ"
+    B, H, T, D = q.shape
+    Hk = k.shape[1]
+    page_table = _pages_arg(name, k_pages, v_pages, page_table, B, Hk, D, q.dtype)
+    _on_device("q", q, k=k, v=v, inv_freq=f, positions=positions, q_weight=wq, k_weight=wk,
+               start=start_dev, k_pages=k_pages, v_pages=v_pages, page_table=page_table)
+    qo = torch.empty_like(q)
+    s = lib.mtp_qk_norm_rope_write(
+        ptr(q), ptr(k), ptr(v), code(q.dtype), B, T, H, Hk, D, *q.stride()[:3], *k.stride()[:3],
+        *v.stride()[:3], ptr(f), int(f.dtype is torch.float64), rot, int(bool(interleaved)),
+        int(bool(norm)), ptr(wq), ptr(wk), float(eps), ptr(positions), pos_sb, ptr(start_dev),
+        per_row, start_host, ptr(qo), *qo.stride()[:3], ptr(k_pages), ptr(v_pages),
+        k_pages.shape[0], k_pages.shape[3], ptr(page_table), page_table.shape[1],
+        _lib.stream_handle(q.device))
+    check(s, name)
+    return qo
+
+
+def _window_arg(name: str, window, sinks) -> Tuple[int, int]:
+    if window is not None and int(window) < 1:
+        raise ValueError(f"{name}: window must be at least 1 (or None), got {window}")
+    if int(sinks) < 0:
+        raise ValueError(f"{name}: sinks must not be negative, got {sinks}")
+    # 2^40 keys are more than any table holds
+    return (-1 if window is None else min(int(window), 1 << 40)), min(int(sinks), 1 << 40)
+
+
+@_on_its_device
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                     window: Optional[int] = None, sinks: int = 0,
+                     lengths: Optional[torch.Tensor] = None,
+                     scale: Optional[float] = None) -> torch.Tensor:
+    """Causal attention of a prompt, or of a chunk behind earlier keys, with a
+    sliding window and first keys that stay visible: query t stands at
+    position p = L - T + t and sees the keys j <= p with p - j < window (None:
+    all) or j < sinks. q [B, H, T, D], k / v [B, Hk, L, D], H a multiple of
+    Hk (query head h reads key head h // (H // Hk)), any strides with d
+    contiguous; lengths [B]: positions from lengths[b] on are padding (keys
+    that nobody sees, rows of zeros). A row that sees no key is zero."""
+    name = "window_attention"
+    lib = _lib.load()
+    assert q.dim() == 4 and k.dim() == 4 and v.shape == k.shape, \
+        f"{name}: q [B, H, T, D], k / v [B, Hk, L, D]"
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    B, H, T, D = q.shape
+    _B, Hk, L, _D = k.shape
+    assert (_B, _D) == (B, D), f"{name}: k / v must be [{B}, Hk, L, {D}], got {tuple(k.shape)}"
+    assert Hk > 0 and H % Hk == 0, f"{name}: {H} query heads over {Hk} key heads"
+    assert T <= L, f"{name}: {T} queries but only {L} keys"
+    assert k.dtype == q.dtype and v.dtype == q.dtype, f"{name}: dtypes differ"
+    win, sinks = _window_arg(name, window, sinks)
+    if lengths is not None:
+        lengths = lengths.contiguous().to(torch.int64)
+        assert tuple(lengths.shape) == (B,), f"{name}: lengths must be [{B}]"
+    _on_device("q", q, k=k, v=v, lengths=lengths)
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    out = torch.empty_like(q)
+    dt = code(q.dtype)
+    nbytes = lib.mtp_window_attention_workspace_bytes(dt, B, H, Hk, T, D, L, win, sinks, 0, 0)
+    ws, stream = _lib.scratch(q, nbytes)
+    s = lib.mtp_window_attention(
+        ptr(q), dt, B, H, Hk, T, D, *q.stride()[:3], ptr(k), *k.stride()[:3], ptr(v),
+        *v.stride()[:3], L, win, sinks, ptr(lengths), float(scale), ptr(out), *out.stride()[:3],
+        ws, nbytes, stream)
+    check(s, name)
+    return out
+
+
+@_on_its_device
+def paged_window_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                           page_table: torch.Tensor, page_size: int, start,
+                           window: Optional[int] = None, sinks: int = 0,
+                           scale: Optional[float] = None,
+                           weights: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """window_attention of the T newest tokens over a paged cache that holds
+    their keys already: query t of row b stands at position start + t (start
+    as in paged_kv_write). q [B, H, T, D], pages [P, B, Hk, page_size, D],
+    page_table [B, L] int32: page of each position, one outside the pool hides
+    its key. A row at a negative position (a padded batch: start = -T) or with
+    no visible key is zero. weights, fp32 [B, Hk, L]: the weight that each key
+    received, summed over the queries and over the heads of its group, is
+    added in place."""
+    name = "paged_window_attention"
+    lib = _lib.load()
+    assert q.dim() == 4, f"{name}: q [B, H, T, D]"
+    q = _rows(q)
+    B, H, T, D = q.shape
+    Hk = k_pages.shape[2] if k_pages.dim() == 5 else 0
+    page_table = _pages_arg(name, k_pages, v_pages, page_table, B, Hk, D, q.dtype)
+    assert k_pages.shape[3] == page_size, f"{name}: pages hold {k_pages.shape[3]} slots"
+    assert Hk > 0 and H % Hk == 0, f"{name}: {H} query heads over {Hk} key heads"
+    L = page_table.shape[1]
+    win, sinks = _window_arg(name, window, sinks)
+    start_dev, per_row, start_host = _start_arg(name, start, B)
+    if weights is not None:
+        assert tuple(weights.shape) == (B, Hk, L) and weights.dtype == torch.float32 and \
+            weights.is_contiguous(), f"{name}: weights must be contiguous float32 [{B}, {Hk}, {L}]"
+    _on_device("q", q, k_pages=k_pages, v_pages=v_pages, page_table=page_table, start=start_dev,
+               weights=weights)
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    out = torch.empty_like(q)
+    dt = code(q.dtype)
+    nbytes = lib.mtp_window_attention_workspace_bytes(dt, B, H, Hk, T, D, L, win, sinks, 1,
+                                                      int(weights is not None))
+    ws, stream = _lib.scratch(q, nbytes)
+    s = lib.mtp_paged_window_attention(
+        ptr(q), dt, B, H, Hk, T, D, *q.stride()[:3], ptr(k_pages), ptr(v_pages), k_pages.shape[0],
+        ptr(page_table), L, int(page_size), ptr(start_dev), per_row, start_host, win, sinks,
+        float(scale), ptr(out), *out.stride()[:3], ptr(weights), ws, nbytes, stream)
+    check(s, name)
+    return out
+
+
+@_on_its_device
+def kv_evict(weights: torch.Tensor, lengths: torch.Tensor, k_pages: torch.Tensor,
+             v_pages: torch.Tensor, page_table: torch.Tensor, out_table: torch.Tensor,
+             sinks: int = 0, recent: int = 0):
+    """Cut a paged cache down by the weight its keys received: each key head
+    of row b keeps, of the first lengths[b] entries of page_table [B, L], its
+    first `sinks`, its last `recent` and the others of largest weight, keep =
+    out_table.shape[1] in all (equal weights: the lower position; NaN is the
+    largest; an entry whose page is outside the pool is never kept). The kept
+    rows are copied in order to the positions 0 .. of out_table [B, keep],
+    whose pages must hold no entry of the same row's page_table. Returns
+    (kept int32 [B, Hk, keep], -1 past the new length; their weights fp32 [B,
+    Hk, keep], 0 past it; new lengths int64 [B]). weights fp32 [B, Hk, L];
+    pages [P, B, Hk, page_size, D] of any dtype; the copied keys keep the
+    rotation they were written with."""
+    name = "kv_evict"
+    lib = _lib.load()
+    assert weights.dim() == 3 and weights.dtype == torch.float32, f"{name}: weights fp32 [B, Hk, L]"
+    weights = weights.contiguous()
+    B, Hk, L = weights.shape
+    assert Hk > 0, f"{name}: no key heads"
+    D = k_pages.shape[-1]
+    assert k_pages.dtype == v_pages.dtype, f"{name}: dtypes differ"
+    page_table = _pages_arg(name, k_pages, v_pages, page_table, B, Hk, D, k_pages.dtype)
+    assert page_table.shape[1] == L, f"{name}: page_table has {page_table.shape[1]} != {L} positions"
+    assert out_table.dim() == 2 and out_table.shape[0] == B and out_table.shape[1] > 0, \
+        f"{name}: out_table must be [{B}, keep]"
+    out_table = _i32(out_table.contiguous())
+    if out_table.numel() and out_table.data_ptr() == page_table.data_ptr():
+        raise ValueError(f"{name}: out_table is page_table: rows cannot move onto themselves")
+    keep = out_table.shape[1]
+    sinks, recent = int(sinks), int(recent)
+    if sinks < 0 or recent < 0 or sinks + recent > keep:
+        raise ValueError(f"{name}: sinks {sinks} and recent {recent} must fit in keep {keep}")
+    lengths = lengths.contiguous().to(torch.int64)
+    assert tuple(lengths.shape) == (B,), f"{name}: lengths must be [{B}]"
+    _on_device("weights", weights, lengths=lengths, k_pages=k_pages, v_pages=v_pages,
+               page_table=page_table, out_table=out_table)
+    dev = weights.device
+    kept = torch.empty((B, Hk, keep), dtype=torch.int32, device=dev)
+    w = torch.empty((B, Hk, keep), dtype=torch.float32, device=dev)
+    n = torch.empty((B,), dtype=torch.int64, device=dev)
+    s = lib.mtp_kv_evict(ptr(weights), ptr(lengths), B, Hk, L, keep, sinks, recent, ptr(k_pages),
+                         ptr(v_pages), k_pages.shape[0], k_pages.shape[3],
+                         D * k_pages.element_size(), ptr(page_table), ptr(out_table), ptr(kept),
+                         ptr(w), ptr(n), _lib.stream_handle(dev))
+    check(s, name)
+    return kept, w, n

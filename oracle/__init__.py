@@ -39,4 +39,7 @@ here, in tests/test_oracle.py):
       row is NaN; paged equals contiguous keys under any page placement;
       the tree-verify step equals one single-query tree_attention call per
       node over context ++ tree keys (how the reference composes it).
+  serving (serving.py; no counterpart in the reference) — brute-force exp
+      sums for the windowed attention and its weights, complex turns for the
+      rotation (tests/test_serving_refusals.py); eviction is a Python sort.
 """
