@@ -10,6 +10,7 @@
 #include "evict.hpp"
 #include "rope.hpp"
 #include "wattn.hpp"
+#include "wattn_weights.hpp"
 
 using namespace mtp;
 
@@ -114,25 +115,55 @@ int rope_args(RopeArgs &a, const void *q, const void *k, int dtype, int64_t B, i
 
 // ---- windowed attention
 struct WinPlan {
-  int64_t ld_sc = 0;
-  size_t ml_off = 0, total = 0;
+  int rt = 0;              // split kernel: row tiles of a block; 0: one wave per row
+  int rblocks = 1, nchunks = 1;
+  int64_t ld_sc = 0;       // scores (with weights)
+  size_t sc_off = 0, ml_off = 0, part_off = 0, pml_off = 0, total = 0;
 };
 
-// Keys that T queries can see of a sequence at most.
-int64_t win_most(int64_t T, int64_t L, int64_t window, int64_t sinks) {
-  if (window < 0 || window >= kWinNone / 2) return L;
-  return std::min(L, std::min(sinks, L) + window + T - 1);
+// Keys that t queries can see of a sequence at most.
+int64_t win_most(int64_t t, int64_t L, int64_t window, int64_t sinks) {
+  if (window == kWinNone) return L;
+  return std::min(L, std::min(sinks, L) + window + t - 1);
 }
 
-WinPlan win_plan(int64_t B, int64_t H, int64_t Hk, int64_t T, int64_t L, int64_t window,
-                 int64_t sinks, bool weights) {
+int win_window(int64_t window) {
+  return window < 0 || window >= kWinNone / 2 ? kWinNone : (int)window;
+}
+
+// Rows of 16 whole bytes at 64 or 128 elements take the split kernel: its
+// workgroups of four waves, two on a CU, and chunks of two steps a wave at
+// least.
+WinPlan win_plan(int dt, int64_t B, int64_t H, int64_t Hk, int64_t T, int64_t D, int64_t L,
+                 int window, int64_t sinks, bool weights) {
   WinPlan p;
-  if (B <= 0 || H <= 0 || Hk <= 0 || T <= 0 || L <= 0) return p;
+  if (B <= 0 || H <= 0 || Hk <= 0 || H % Hk != 0 || T <= 0 || L <= 0) return p;
+  const int64_t rows = H / Hk * T, units = B * Hk;
+  size_t at = kCounterBytes;
+  if (win_split_pick(dt, (int)std::min<int64_t>(D, 1 << 20), 1, false)) {
+    p.rt = rows > 16 ? 2 : 1;
+    const int64_t rp = 16 * p.rt;
+    p.rblocks = (int)((rows + rp - 1) / rp);
+    const int64_t most = win_most(std::min(T, (rp - 1) / (H / Hk) + 2), L, window, sinks);
+    const int64_t step = (int64_t)kWinSplitWaves * win_split_keys((int)D * dtype_bytes(dt));
+    const int64_t room = 2 * (int64_t)device_cus() / (units * p.rblocks);
+    p.nchunks = (int)std::max<int64_t>(1, std::min(room, most / (2 * step)));
+    if (p.nchunks > 1) {
+      const int64_t parts = units * p.rblocks * p.nchunks * rp;
+      p.part_off = at;
+      at += align_up((size_t)parts * (size_t)D * 4, 256);
+      p.pml_off = at;
+      at += align_up((size_t)parts * 8, 256);
+    }
+  }
   if (weights) {
     p.ld_sc = win_most(T, L, window, sinks);
-    p.ml_off = kCounterBytes + align_up((size_t)(B * H * T) * (size_t)p.ld_sc * 4, 256);
-    p.total = p.ml_off + align_up((size_t)(B * H * T) * 8, 256);
+    p.sc_off = at;
+    at += align_up((size_t)(B * H * T) * (size_t)p.ld_sc * 4, 256);
+    p.ml_off = at;
+    at += align_up((size_t)(B * H * T) * 8, 256);
   }
+  p.total = at > kCounterBytes ? at : 0;
   return p;
 }
 
@@ -146,22 +177,44 @@ void (*win_generic(int64_t d))(WinArgs, int) {
 constexpr int64_t kWinMaxD = 1024;
 
 int win_launch(WinArgs &a, int dt, void *workspace, size_t workspace_bytes, hipStream_t st) {
-  const WinPlan p = win_plan(a.B, a.H, a.Hk, a.T, a.L, a.window == kWinNone ? -1 : a.window,
-                             a.sinks, a.weights != nullptr);
+  const WinPlan p = win_plan(dt, a.B, a.H, a.Hk, a.T, a.D, a.L, a.window, a.sinks,
+                             a.weights != nullptr);
   if (p.total > 0 && (!workspace || workspace_bytes < p.total)) return MTP_ERR_WORKSPACE;
+  const int64_t rows = (int64_t)a.B * a.H * a.T;
+  if (rows > INT32_MAX) return MTP_ERR_SHAPE;
   unsigned char *const w8 = (unsigned char *)workspace;
   if (a.weights) {
-    a.scores = (float *)(w8 + kCounterBytes);
+    a.scores = (float *)(w8 + p.sc_off);
     a.ld_sc = p.ld_sc;
     a.ml = (float *)(w8 + p.ml_off);
   }
-  const int64_t rows = (int64_t)a.B * a.H * a.T;
-  if (rows > INT32_MAX) return MTP_ERR_SHAPE;
-  hipLaunchKernelGGL(a.table ? win_generic<true>(a.D) : win_generic<false>(a.D),
-                     dim3((unsigned)rows), dim3(64), win_row_lds(a.D) * 4, st, a, dt);
-  const int s = launch_status();
+  const int64_t e = 16 / dtype_bytes(dt);
+  const bool whole = aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.out) &&
+                     mult({a.q_sb, a.q_sh, a.q_st, a.k_sb, a.k_sh, a.k_st, a.v_sb, a.v_sh, a.v_st,
+                           a.o_sb, a.o_sh, a.o_st, a.p_sp},
+                          e);
+  int s;
+  if (p.rt && whole && p.rblocks <= 65535) {
+    a.rblocks = p.rblocks;
+    a.nchunks = p.nchunks;
+    a.part = (float *)(w8 + p.part_off);
+    a.pml = (float *)(w8 + p.pml_off);
+    const bool paged = a.table != nullptr;
+    hipLaunchKernelGGL(win_split_pick(dt, a.D, p.rt, paged),
+                       dim3((unsigned)(a.B * a.Hk), (unsigned)p.rblocks, (unsigned)p.nchunks),
+                       dim3(64 * kWinSplitWaves), 0, st, a);
+    s = launch_status();
+    if (s == MTP_OK && p.nchunks > 1) {
+      hipLaunchKernelGGL(win_merge_pick(dt, a.D, p.rt, paged), dim3((unsigned)((rows + 3) / 4)),
+                         dim3(256), 0, st, a);
+      s = launch_status();
+    }
+  } else {
+    hipLaunchKernelGGL(a.table ? win_generic<true>(a.D) : win_generic<false>(a.D),
+                       dim3((unsigned)rows), dim3(64), win_row_lds(a.D) * 4, st, a, dt);
+    s = launch_status();
+  }
   if (s != MTP_OK || !a.weights) return s;
-  if ((int64_t)a.B * a.Hk > 65535) return MTP_ERR_SHAPE;
   hipLaunchKernelGGL(win_weights_kernel, dim3((unsigned)((p.ld_sc + 255) / 256),
                                               (unsigned)(a.B * a.Hk)),
                      dim3(256), 0, st, a);
@@ -197,7 +250,7 @@ int win_args(WinArgs &a, const void *q, int dtype, int64_t B, int64_t H, int64_t
   a.T = (int)T;
   a.D = (int)D;
   a.L = (int)L;
-  a.window = window < 0 || window >= kWinNone / 2 ? kWinNone : (int)window;
+  a.window = win_window(window);
   a.sinks = (int)std::min(sinks, L);
   a.scale = scale * 1.44269504088896340736f;
   a.nchunks = 1;
@@ -271,8 +324,12 @@ int mtp_qk_norm_rope_write(const void *q, const void *k, const void *v, int dtyp
 size_t mtp_window_attention_workspace_bytes(int dtype, int64_t B, int64_t H, int64_t Hk, int64_t T,
                                             int64_t D, int64_t L, int64_t window, int64_t sinks,
                                             int paged, int weights) {
-  (void)dtype, (void)D, (void)paged;
-  return win_plan(B, H, Hk, T, L, window, sinks, weights != 0).total;
+  (void)paged;
+  if (!is_float_dt(dtype) || T > kWinMaxKeys || L > kWinMaxKeys || B > INT32_MAX || H > 65535)
+    return 0;
+  return win_plan(dtype, B, H, Hk, T, D, L, win_window(window), std::max<int64_t>(sinks, 0),
+                  weights != 0)
+      .total;
 }
 
 int mtp_window_attention(const void *q, int dtype, int64_t B, int64_t H, int64_t Hk, int64_t T,

@@ -20,7 +20,9 @@
 
 namespace mtp {
 
-__device__ __forceinline__ WinSpan win_span(const WinArgs &a, int b) {
+// The span of the rows t0 .. t1 - 1 of sequence b; first and rows are those of
+// the whole call.
+__device__ __forceinline__ WinSpan win_span(const WinArgs &a, int b, int t0, int t1) {
   WinSpan s;
   const int64_t st = a.start_dev ? a.start_dev[a.start_per_row ? b : 0] : a.start_host;
   // past L + window every start sees the same keys: none but the sinks, or
@@ -33,11 +35,16 @@ __device__ __forceinline__ WinSpan win_span(const WinArgs &a, int b) {
     end = (int)min(max(a.lengths[b], (int64_t)0), (int64_t)a.L);
     s.rows = min(a.T, max(0, end - s.first));
   }
-  s.hi = max(0, min(end, s.first + s.rows));
-  s.lo = a.window == kWinNone ? 0 : max(0, s.first - a.window + 1);
+  t1 = min(t1, s.rows);
+  s.hi = t0 < t1 ? max(0, min(end, s.first + t1)) : 0;
+  s.lo = a.window == kWinNone ? 0 : max(0, s.first + t0 - a.window + 1);
   s.ns = min(min(a.sinks, s.lo), s.hi);
   s.lo = min(max(s.lo, s.ns), s.hi);
   return s;
+}
+
+__device__ __forceinline__ WinSpan win_span(const WinArgs &a, int b) {
+  return win_span(a, b, 0, a.T);
 }
 
 // Whether the row at position pos sees key j (j below the span's end).
@@ -59,6 +66,21 @@ __device__ __forceinline__ bool win_key_at(const WinArgs &a, int b, int hk, int 
     ko = (int64_t)b * a.k_sb + (int64_t)hk * a.k_sh + (int64_t)j * a.k_st;
     vo = (int64_t)b * a.v_sb + (int64_t)hk * a.v_sh + (int64_t)j * a.v_st;
     return true;
+  }
+}
+
+// Four elements from d on of row (b, h, t) of the output; CT's 4-element rows
+// are aligned (o strides and address in whole 16 bytes).
+template <int CT>
+__device__ __forceinline__ void win_store4(const WinArgs &a, int b, int h, int t, int d, f32x4 v) {
+  const int64_t at = (int64_t)b * a.o_sb + (int64_t)h * a.o_sh + (int64_t)t * a.o_st + d;
+  if constexpr (CT == MTP_F32) {
+    *(f32x4 *)((float *)a.out + at) = v;
+  } else {
+    uint2 w;
+    w.x = pack2<CT>(v[0], v[1]);
+    w.y = pack2<CT>(v[2], v[3]);
+    *(uint2 *)((uint16_t *)a.out + at) = w;
   }
 }
 
@@ -148,39 +170,6 @@ __global__ void __launch_bounds__(64) win_rows_generic_kernel(const WinArgs a, i
   const int h = (int)((r / a.T) % a.H);
   const int b = (int)(r / ((int64_t)a.T * a.H));
   win_row<NV, PAGED>(a, ct, b, h, t, win_span(a, b), s_row, a.scores != nullptr);
-}
-
-// The weight of every key that a query saw, added to a.weights: sum over the
-// rows of the key's head of exp2(score - max) / sum, rows in order, so the
-// result does not depend on timing. Grid (keys / 256, B * Hk).
-__global__ void __launch_bounds__(256) win_weights_kernel(const WinArgs a) {
-  __shared__ float s_m[256], s_i[256];
-  const int bh = blockIdx.y, b = bh / a.Hk;
-  const WinSpan s = win_span(a, b);
-  const int n = s.count();
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if ((int)blockIdx.x * 256 >= n) return;  // the whole workgroup
-  const int rows = a.G * a.T;
-  float w = 0.f;
-  for (int r0 = 0; r0 < rows; r0 += 256) {
-    const int r = r0 + threadIdx.x;
-    __syncthreads();
-    if (r < rows) {
-      const float *const ml = a.ml + ((int64_t)bh * rows + r) * 2;
-      const float m = ml[0], l = ml[1];
-      s_m[threadIdx.x] = m == -INFINITY ? 0.f : m;
-      s_i[threadIdx.x] = l == 0.f ? 0.f : 1.f / l;
-    }
-    __syncthreads();
-    if (i < n) {
-      const int most = min(256, rows - r0);
-      const float *const sc = a.scores + ((int64_t)bh * rows + r0) * a.ld_sc + i;
-      for (int r = 0; r < most; ++r)
-        if (r0 + r < s.rows * a.G)  // rows of no query keep no scores
-          w = fmaf(__builtin_amdgcn_exp2f(sc[(int64_t)r * a.ld_sc] - s_m[r]), s_i[r], w);
-    }
-  }
-  if (i < n) a.weights[(int64_t)bh * a.L + s.key(i)] += w;
 }
 
 }  // namespace mtp

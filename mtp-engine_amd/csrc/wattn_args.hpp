@@ -35,9 +35,10 @@ struct WinArgs {
   float *ml;                      // [B * Hk][G * T][2]: maximum and sum of a row, with scores
   int64_t ld_sc;
   float *weights;                 // [B, Hk, L], added to
-  int nchunks;                    // key chunks of a (batch, key head, row block)
-  float *part;                    // [unit][chunk][rows][D + 2] partials, nchunks > 1
-  unsigned *ticket;               // arrivals per unit
+  // split kernel: row blocks of a (batch, key head), key chunks of a block
+  int rblocks, nchunks;
+  float *part;                    // [b * Hk + hk][row block][chunk][rows][D], nchunks > 1
+  float *pml;                     // the same with (maximum, sum) for D
 };
 
 // The keys that the queries of one sequence see: [0, ns) and [lo, hi), the
@@ -47,8 +48,21 @@ struct WinArgs {
 struct WinSpan {
   int first, rows, ns, lo, hi;
   __host__ __device__ int count() const { return ns + hi - lo; }
-  // Key of compact index i < count().
+  // Key of compact index i < count(), and back.
   __host__ __device__ int key(int i) const { return i < ns ? i : lo + (i - ns); }
+  __host__ __device__ int index(int j) const { return j < ns ? j : j - lo + ns; }
 };
+
+// Rows of the split kernel's tiles and its waves; see wattn_split.hpp.
+constexpr int kWinSplitWaves = 4;
+// Keys of a wave's step: whole K = 32 products (16-bit types), and at most 8
+// KB of K.
+constexpr int win_split_keys(int row_bytes) { return row_bytes > 256 ? 16 : 32; }
+
+typedef void (*WinKernel)(WinArgs);
+// The split kernel for rows of type ct and head dim d in tiles of 16 * rt rows
+// (rt 1 or 2) and the merge of its chunks; null for other shapes.
+WinKernel win_split_pick(int ct, int d, int rt, bool paged);
+WinKernel win_merge_pick(int ct, int d, int rt, bool paged);
 
 }  // namespace mtp
