@@ -194,7 +194,19 @@ int win_launch(WinArgs &a, int dt, void *workspace, size_t workspace_bytes, hipS
                            a.o_sb, a.o_sh, a.o_st, a.p_sp},
                           e);
   int s;
-  if (p.rt && whole && p.rblocks <= 65535) {
+  // the prompt kernel: dense keys whose rows a buffer's 32-bit offsets reach
+  const int64_t reach = ((int64_t)1 << 31) / 2 - a.D;
+  const bool near = a.k_st >= 0 && a.v_st >= 0 && (a.L - 1) * a.k_st < reach &&
+                    (a.L - 1) * a.v_st < reach;
+  const int nw = 8;
+  const WinKernel prompt = a.table || !near ? nullptr : win_prompt_pick(dt, a.D, nw);
+  const int64_t pblocks = ((int64_t)a.G * a.T + 32 * nw - 1) / (32 * nw);
+  if (prompt && whole && (int64_t)a.G * a.T > 128 && pblocks <= 65535) {
+    a.rblocks = (int)pblocks;
+    hipLaunchKernelGGL(prompt, dim3((unsigned)(a.B * a.Hk), (unsigned)pblocks), dim3(64 * nw),
+                       win_prompt_lds(a.D), st, a);
+    s = launch_status();
+  } else if (p.rt && whole && p.rblocks <= 65535) {
     a.rblocks = p.rblocks;
     a.nchunks = p.nchunks;
     a.part = (float *)(w8 + p.part_off);

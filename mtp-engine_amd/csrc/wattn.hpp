@@ -49,7 +49,7 @@ __device__ __forceinline__ WinSpan win_span(const WinArgs &a, int b) {
 
 // Whether the row at position pos sees key j (j below the span's end).
 __device__ __forceinline__ bool win_sees(const WinArgs &a, int pos, int j) {
-  return j <= pos && (j > pos - a.window || j < a.sinks);
+  return (j <= pos) & ((j > pos - a.window) | (j < a.sinks));  // no branches
 }
 
 // Element offset of key j's row in k (and, dense, by its own strides in v), or

@@ -65,4 +65,11 @@ typedef void (*WinKernel)(WinArgs);
 WinKernel win_split_pick(int ct, int d, int rt, bool paged);
 WinKernel win_merge_pick(int ct, int d, int rt, bool paged);
 
+// The prompt kernel (wattn_prompt.hpp) for 16-bit rows of head dim d in blocks
+// of 32 * nw rows (nw 4 or 8), and the keys of its tiles; null for other
+// shapes. Grid (B * Hk, row blocks).
+constexpr int kWinTileKeys = 64;
+WinKernel win_prompt_pick(int ct, int d, int nw);
+constexpr int win_prompt_lds(int d) { return 2 * 2 * kWinTileKeys * 2 * d; }
+
 }  // namespace mtp

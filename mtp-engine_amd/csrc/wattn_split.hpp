@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(64 * kWinSplitWaves, 2) win_split_kernel(const
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int j = s.key(i0 + 16 * kt + 4 * g + i);
-            const bool see = ((okm >> (16 * kt + 4 * g + i)) & 1u) && win_sees(a, pos[rt], j);
+            const bool see = (((okm >> (16 * kt + 4 * g + i)) & 1u) != 0) & win_sees(a, pos[rt], j);
             sc[rt][kt][i] = see ? sc[rt][kt][i] : -INFINITY;
           }
         }
