@@ -594,17 +594,21 @@ int mtp_batch_prefix_match(const int64_t *ids, int64_t R, int64_t L,
  * NULL; start as in mtp_paged_kv_write. The angle is reduced in 64 bits;
  * everything else is fp32, rounded once.
  */
-int mtp_qk_norm_rope(const void *q, const void *k, int dtype, int64_t B,
-                     int64_t T, int64_t H, int64_t Hk, int64_t D, int64_t q_sb,
-                     int64_t q_sh, int64_t q_st, int64_t k_sb, int64_t k_sh,
-                     int64_t k_st, const void *inv_freq, int freq_f64,
-                     int64_t rot, int interleaved, int norm,
-                     const float *q_weight, const float *k_weight, float eps,
-                     const int64_t *positions, int64_t pos_sb,
-                     const int64_t *start_dev, int start_per_row,
-                     int64_t start_host, void *q_out, int64_t qo_sb,
-                     int64_t qo_sh, int64_t qo_st, void *k_out, int64_t ko_sb,
-                     int64_t ko_sh, int64_t ko_st, void *stream);
+typedef struct mtp_rope_args {
+  const void *q, *k, *v;          /* v, pages, page_table: _write alone */
+  void *q_out, *k_out;            /* k_out: not with _write */
+  void *k_pages, *v_pages;
+  const int32_t *page_table;
+  const void *inv_freq;
+  const float *q_weight, *k_weight;
+  const int64_t *positions, *start_dev;
+  int64_t B, T, H, Hk, D;
+  int64_t q_st[3], k_st[3], v_st[3], qo_st[3], ko_st[3]; /* batch, head, token */
+  int64_t rot, pos_sb, start_host, num_pages, page_size, ld_tab;
+  float eps;
+  int32_t dtype, freq_f64, interleaved, norm, start_per_row;
+} mtp_rope_args;
+int mtp_qk_norm_rope(const mtp_rope_args *args, void *stream);
 
 /*
  * The same, with the keys written into their pages beside the values v [B,
@@ -613,17 +617,7 @@ int mtp_qk_norm_rope(const void *q, const void *k, int dtype, int64_t B,
  * outside [0, num_pages) are skipped). Pages [num_pages, B, Hk, page_size, D]
  * in dtype; page_table [B, ld_tab] int32.
  */
-int mtp_qk_norm_rope_write(
-    const void *q, const void *k, const void *v, int dtype, int64_t B,
-    int64_t T, int64_t H, int64_t Hk, int64_t D, int64_t q_sb, int64_t q_sh,
-    int64_t q_st, int64_t k_sb, int64_t k_sh, int64_t k_st, int64_t v_sb,
-    int64_t v_sh, int64_t v_st, const void *inv_freq, int freq_f64, int64_t rot,
-    int interleaved, int norm, const float *q_weight, const float *k_weight,
-    float eps, const int64_t *positions, int64_t pos_sb,
-    const int64_t *start_dev, int start_per_row, int64_t start_host,
-    void *q_out, int64_t qo_sb, int64_t qo_sh, int64_t qo_st, void *k_pages,
-    void *v_pages, int64_t num_pages, int64_t page_size,
-    const int32_t *page_table, int64_t ld_tab, void *stream);
+int mtp_qk_norm_rope_write(const mtp_rope_args *args, void *stream);
 
 /*
  * Attention of a prompt (or of a chunk behind earlier keys) with a sliding
@@ -638,16 +632,22 @@ int mtp_qk_norm_rope_write(
  * lengths[b] are padding: such keys are never read, such rows are zero. A row
  * that sees no key is zero.
  */
-int mtp_window_attention(const void *q, int dtype, int64_t B, int64_t H,
-                         int64_t Hk, int64_t T, int64_t D, int64_t q_sb,
-                         int64_t q_sh, int64_t q_st, const void *k,
-                         int64_t k_sb, int64_t k_sh, int64_t k_st,
-                         const void *v, int64_t v_sb, int64_t v_sh,
-                         int64_t v_st, int64_t L, int64_t window,
-                         int64_t sinks, const int64_t *lengths, float scale,
-                         void *out, int64_t o_sb, int64_t o_sh, int64_t o_st,
-                         void *workspace, size_t workspace_bytes,
-                         void *stream);
+typedef struct mtp_window_args {
+  const void *q, *k, *v;          /* paged: k, v are the pages */
+  void *out;
+  const int32_t *page_table;      /* page_table, start_dev, weights: paged alone */
+  const int64_t *start_dev;
+  const int64_t *lengths;         /* dense alone */
+  float *weights;
+  void *workspace;
+  size_t workspace_bytes;
+  int64_t B, H, Hk, T, D, L;
+  int64_t q_st[3], k_st[3], v_st[3], out_st[3]; /* batch, head, token; k_st, v_st dense alone */
+  int64_t window, sinks, start_host, num_pages, page_size;
+  float scale;
+  int32_t dtype, start_per_row;
+} mtp_window_args;
+int mtp_window_attention(const mtp_window_args *args, void *stream);
 
 /*
  * The same for a few new tokens whose keys are in the paged cache already:
@@ -660,14 +660,7 @@ int mtp_window_attention(const void *q, int dtype, int64_t B, int64_t H,
  * this call's queries is added, summed over the T queries and the H / Hk
  * heads of its key head.
  */
-int mtp_paged_window_attention(
-    const void *q, int dtype, int64_t B, int64_t H, int64_t Hk, int64_t T,
-    int64_t D, int64_t q_sb, int64_t q_sh, int64_t q_st, const void *k_pages,
-    const void *v_pages, int64_t num_pages, const int32_t *page_table,
-    int64_t L, int64_t page_size, const int64_t *start_dev, int start_per_row,
-    int64_t start_host, int64_t window, int64_t sinks, float scale, void *out,
-    int64_t o_sb, int64_t o_sh, int64_t o_st, float *weights, void *workspace,
-    size_t workspace_bytes, void *stream);
+int mtp_paged_window_attention(const mtp_window_args *args, void *stream);
 
 /* Workspace bytes of the two entry points above (paged = 0 / 1; weights = 1
  * where the paged one is given weights). */

@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cstddef>
 
 #include "abi_util.hpp"
 #include "evict.hpp"
@@ -13,6 +14,11 @@
 #include "wattn_weights.hpp"
 
 using namespace mtp;
+
+// The layouts that mtp_hip/_lib.py packs.
+static_assert(sizeof(mtp_rope_args) == 336 && offsetof(mtp_rope_args, eps) == 312, "mtp_rope_args");
+static_assert(sizeof(mtp_window_args) == 280 && offsetof(mtp_window_args, scale) == 264,
+              "mtp_window_args");
 
 namespace {
 
@@ -62,15 +68,17 @@ RopeKernel rope_pick(const RopeArgs &a, int dt, int &lpr) {
 int rope_launch(RopeArgs &a, int dt, hipStream_t st) {
   int lpr = 0;
   const int64_t toks = (int64_t)a.B * a.T;
-  const int64_t nr = a.H + a.Hk + (a.v ? a.Hk : 0);
   if (RopeKernel k = rope_pick(a, dt, lpr)) {
-    // a wave per token, more of them while the chip has room
+    // a wave per token, more of them while the chip has room: up to one for
+    // every 64 / lpr rows
     const int64_t rpi = 64 / lpr, room = (int64_t)device_cus() * 8;
-    a.hs = (int)std::max<int64_t>(1, std::min((room + toks - 1) / toks, (nr + rpi - 1) / rpi));
+    const int64_t most = (a.H + rpi - 1) / rpi + (a.v ? 2 : 1) * ((a.Hk + rpi - 1) / rpi);
+    a.hs = (int)std::max<int64_t>(1, std::min((room + toks - 1) / toks, most));
     const int64_t blocks = (toks * a.hs + 3) / 4;
     if (blocks > INT32_MAX) return MTP_ERR_SHAPE;
     hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(256), 0, st, a);
   } else {
+    const int64_t nr = a.H + a.Hk + (a.v ? a.Hk : 0);
     if (toks * nr > INT32_MAX) return MTP_ERR_SHAPE;
     hipLaunchKernelGGL(rope_generic_kernel, dim3((unsigned)(toks * nr)), dim3(64), 0, st, a, dt);
   }
@@ -78,38 +86,40 @@ int rope_launch(RopeArgs &a, int dt, hipStream_t st) {
 }
 
 // What both entry points check and fill in; > 0: nothing to do.
-int rope_args(RopeArgs &a, const void *q, const void *k, int dtype, int64_t B, int64_t T, int64_t H,
-              int64_t Hk, int64_t D, const void *inv_freq, int freq_f64, int64_t rot,
-              int interleaved, int norm, const float *q_weight, const float *k_weight, float eps,
-              const int64_t *positions, int64_t pos_sb, const int64_t *start_dev,
-              int start_per_row, int64_t start_host, void *q_out) {
-  if (!is_float_dt(dtype)) return MTP_ERR_DTYPE;
+int rope_args(RopeArgs &a, const mtp_rope_args *p) {
+  if (!p) return MTP_ERR_NULL;
+  if (!is_float_dt(p->dtype)) return MTP_ERR_DTYPE;
+  const int64_t B = p->B, T = p->T, H = p->H, Hk = p->Hk, D = p->D, rot = p->rot;
   if (B < 0 || T < 0 || H < 0 || Hk < 0 || D <= 0 || D > kRopeMaxD || rot < 0 || rot > D ||
       rot % 2 != 0 || B > INT32_MAX || T > INT32_MAX || H > 65535 || Hk > 65535)
     return MTP_ERR_SHAPE;
   if (B == 0 || T == 0 || H + Hk == 0) return 1;
-  if ((H > 0 && (!q || !q_out)) || (Hk > 0 && !k) || (rot > 0 && !inv_freq)) return MTP_ERR_NULL;
-  a.q = q;
-  a.k = k;
-  a.qo = q_out;
-  a.inv_freq = inv_freq;
-  a.freq64 = freq_f64 ? 1 : 0;
-  a.wq = q_weight;
-  a.wk = k_weight;
-  a.pos = positions;
-  a.pos_sb = pos_sb;
-  a.start_dev = start_dev;
-  a.start_per_row = start_per_row ? 1 : 0;
-  a.start_host = start_host;
+  if ((H > 0 && (!p->q || !p->q_out)) || (Hk > 0 && !p->k) || (rot > 0 && !p->inv_freq))
+    return MTP_ERR_NULL;
+  a.q = p->q;
+  a.k = p->k;
+  a.qo = p->q_out;
+  a.q_sb = p->q_st[0], a.q_sh = p->q_st[1], a.q_st = p->q_st[2];
+  a.k_sb = p->k_st[0], a.k_sh = p->k_st[1], a.k_st = p->k_st[2];
+  a.qo_sb = p->qo_st[0], a.qo_sh = p->qo_st[1], a.qo_st = p->qo_st[2];
+  a.inv_freq = p->inv_freq;
+  a.freq64 = p->freq_f64 ? 1 : 0;
+  a.wq = p->q_weight;
+  a.wk = p->k_weight;
+  a.pos = p->positions;
+  a.pos_sb = p->pos_sb;
+  a.start_dev = p->start_dev;
+  a.start_per_row = p->start_per_row ? 1 : 0;
+  a.start_host = p->start_host;
   a.B = (int)B;
   a.T = (int)T;
   a.H = (int)H;
   a.Hk = (int)Hk;
   a.D = (int)D;
   a.rot = (int)rot;
-  a.norm = norm ? 1 : 0;
-  a.interleaved = interleaved ? 1 : 0;
-  a.eps = eps;
+  a.norm = p->norm ? 1 : 0;
+  a.interleaved = p->interleaved ? 1 : 0;
+  a.eps = p->eps;
   return MTP_OK;
 }
 
@@ -234,27 +244,22 @@ int win_launch(WinArgs &a, int dt, void *workspace, size_t workspace_bytes, hipS
 }
 
 // What both entry points check and fill in; > 0: nothing to do.
-int win_args(WinArgs &a, const void *q, int dtype, int64_t B, int64_t H, int64_t Hk, int64_t T,
-             int64_t D, int64_t q_sb, int64_t q_sh, int64_t q_st, const void *k, const void *v,
-             int64_t L, int64_t window, int64_t sinks, float scale, void *out, int64_t o_sb,
-             int64_t o_sh, int64_t o_st) {
-  if (!is_float_dt(dtype)) return MTP_ERR_DTYPE;
+int win_args(WinArgs &a, const mtp_window_args *p) {
+  if (!p) return MTP_ERR_NULL;
+  if (!is_float_dt(p->dtype)) return MTP_ERR_DTYPE;
+  const int64_t B = p->B, H = p->H, Hk = p->Hk, T = p->T, D = p->D, L = p->L;
   if (B < 0 || T < 0 || H < 0 || Hk <= 0 || H % Hk != 0 || D <= 0 || D > kWinMaxD || L < 0 ||
       B > INT32_MAX || H > 65535 || T > kWinMaxKeys || L > kWinMaxKeys)
     return MTP_ERR_SHAPE;
-  if (window == 0 || window < -1 || sinks < 0) return MTP_ERR_ARG;
+  if (p->window == 0 || p->window < -1 || p->sinks < 0) return MTP_ERR_ARG;
   if (B == 0 || T == 0 || H == 0) return 1;
-  if (!q || !out || (L > 0 && (!k || !v))) return MTP_ERR_NULL;
-  a.q = q;
-  a.q_sb = q_sb;
-  a.q_sh = q_sh;
-  a.q_st = q_st;
-  a.k = k;
-  a.v = v;
-  a.out = out;
-  a.o_sb = o_sb;
-  a.o_sh = o_sh;
-  a.o_st = o_st;
+  if (!p->q || !p->out || (L > 0 && (!p->k || !p->v))) return MTP_ERR_NULL;
+  a.q = p->q;
+  a.q_sb = p->q_st[0], a.q_sh = p->q_st[1], a.q_st = p->q_st[2];
+  a.k = p->k;
+  a.v = p->v;
+  a.out = p->out;
+  a.o_sb = p->out_st[0], a.o_sh = p->out_st[1], a.o_st = p->out_st[2];
   a.B = (int)B;
   a.H = (int)H;
   a.Hk = (int)Hk;
@@ -262,9 +267,9 @@ int win_args(WinArgs &a, const void *q, int dtype, int64_t B, int64_t H, int64_t
   a.T = (int)T;
   a.D = (int)D;
   a.L = (int)L;
-  a.window = win_window(window);
-  a.sinks = (int)std::min(sinks, L);
-  a.scale = scale * 1.44269504088896340736f;
+  a.window = win_window(p->window);
+  a.sinks = (int)std::min(p->sinks, L);
+  a.scale = p->scale * 1.44269504088896340736f;
   a.nchunks = 1;
   return MTP_OK;
 }
@@ -273,64 +278,39 @@ int win_args(WinArgs &a, const void *q, int dtype, int64_t B, int64_t H, int64_t
 
 extern "C" {
 
-int mtp_qk_norm_rope(const void *q, const void *k, int dtype, int64_t B, int64_t T, int64_t H,
-                     int64_t Hk, int64_t D, int64_t q_sb, int64_t q_sh, int64_t q_st, int64_t k_sb,
-                     int64_t k_sh, int64_t k_st, const void *inv_freq, int freq_f64, int64_t rot,
-                     int interleaved, int norm, const float *q_weight, const float *k_weight,
-                     float eps, const int64_t *positions, int64_t pos_sb, const int64_t *start_dev,
-                     int start_per_row, int64_t start_host, void *q_out, int64_t qo_sb,
-                     int64_t qo_sh, int64_t qo_st, void *k_out, int64_t ko_sb, int64_t ko_sh,
-                     int64_t ko_st, void *stream) {
+int mtp_qk_norm_rope(const mtp_rope_args *p, void *stream) {
   RopeArgs a{};
-  const int s = rope_args(a, q, k, dtype, B, T, H, Hk, D, inv_freq, freq_f64, rot, interleaved,
-                          norm, q_weight, k_weight, eps, positions, pos_sb, start_dev,
-                          start_per_row, start_host, q_out);
+  const int s = rope_args(a, p);
   if (s != MTP_OK) return s > 0 ? MTP_OK : s;
-  if (Hk > 0 && !k_out) return MTP_ERR_NULL;
-  a.q_sb = q_sb, a.q_sh = q_sh, a.q_st = q_st;
-  a.k_sb = k_sb, a.k_sh = k_sh, a.k_st = k_st;
-  a.qo_sb = qo_sb, a.qo_sh = qo_sh, a.qo_st = qo_st;
-  a.ko = k_out;
-  a.ko_sb = ko_sb, a.ko_sh = ko_sh, a.ko_st = ko_st;
-  return rope_launch(a, dtype, (hipStream_t)stream);
+  if (p->Hk > 0 && !p->k_out) return MTP_ERR_NULL;
+  a.ko = p->k_out;
+  a.ko_sb = p->ko_st[0], a.ko_sh = p->ko_st[1], a.ko_st = p->ko_st[2];
+  return rope_launch(a, p->dtype, (hipStream_t)stream);
 }
 
-int mtp_qk_norm_rope_write(const void *q, const void *k, const void *v, int dtype, int64_t B,
-                           int64_t T, int64_t H, int64_t Hk, int64_t D, int64_t q_sb, int64_t q_sh,
-                           int64_t q_st, int64_t k_sb, int64_t k_sh, int64_t k_st, int64_t v_sb,
-                           int64_t v_sh, int64_t v_st, const void *inv_freq, int freq_f64,
-                           int64_t rot, int interleaved, int norm, const float *q_weight,
-                           const float *k_weight, float eps, const int64_t *positions,
-                           int64_t pos_sb, const int64_t *start_dev, int start_per_row,
-                           int64_t start_host, void *q_out, int64_t qo_sb, int64_t qo_sh,
-                           int64_t qo_st, void *k_pages, void *v_pages, int64_t num_pages,
-                           int64_t page_size, const int32_t *page_table, int64_t ld_tab,
-                           void *stream) {
+int mtp_qk_norm_rope_write(const mtp_rope_args *p, void *stream) {
   RopeArgs a{};
-  const int s = rope_args(a, q, k, dtype, B, T, H, Hk, D, inv_freq, freq_f64, rot, interleaved,
-                          norm, q_weight, k_weight, eps, positions, pos_sb, start_dev,
-                          start_per_row, start_host, q_out);
+  const int s = rope_args(a, p);
   if (s < 0) return s;
-  if (num_pages < 0 || page_size <= 0 || ld_tab < 0 || num_pages > INT32_MAX ||
-      page_size > INT32_MAX)
+  if (p->num_pages < 0 || p->page_size <= 0 || p->ld_tab < 0 || p->num_pages > INT32_MAX ||
+      p->page_size > INT32_MAX)
     return MTP_ERR_SHAPE;
   if (s > 0) return MTP_OK;
-  if (Hk > 0 && (!v || !k_pages || !v_pages || (ld_tab > 0 && !page_table))) return MTP_ERR_NULL;
-  a.q_sb = q_sb, a.q_sh = q_sh, a.q_st = q_st;
-  a.k_sb = k_sb, a.k_sh = k_sh, a.k_st = k_st;
-  a.v = v;
-  a.v_sb = v_sb, a.v_sh = v_sh, a.v_st = v_st;
-  a.qo_sb = qo_sb, a.qo_sh = qo_sh, a.qo_st = qo_st;
-  a.k_pages = k_pages;
-  a.v_pages = v_pages;
-  a.p_sh = page_size * D;
-  a.p_sb = Hk * a.p_sh;
-  a.p_sp = B * a.p_sb;
-  a.table = page_table;
-  a.ld_tab = ld_tab;
-  a.page_size = (int)page_size;
-  a.npages = (int)num_pages;
-  return rope_launch(a, dtype, (hipStream_t)stream);
+  if (p->Hk > 0 &&
+      (!p->v || !p->k_pages || !p->v_pages || (p->ld_tab > 0 && !p->page_table)))
+    return MTP_ERR_NULL;
+  a.v = p->v;
+  a.v_sb = p->v_st[0], a.v_sh = p->v_st[1], a.v_st = p->v_st[2];
+  a.k_pages = p->k_pages;
+  a.v_pages = p->v_pages;
+  a.p_sh = p->page_size * p->D;
+  a.p_sb = p->Hk * a.p_sh;
+  a.p_sp = p->B * a.p_sb;
+  a.table = p->page_table;
+  a.ld_tab = p->ld_tab;
+  a.page_size = (int)p->page_size;
+  a.npages = (int)p->num_pages;
+  return rope_launch(a, p->dtype, (hipStream_t)stream);
 }
 
 size_t mtp_window_attention_workspace_bytes(int dtype, int64_t B, int64_t H, int64_t Hk, int64_t T,
@@ -344,57 +324,42 @@ size_t mtp_window_attention_workspace_bytes(int dtype, int64_t B, int64_t H, int
       .total;
 }
 
-int mtp_window_attention(const void *q, int dtype, int64_t B, int64_t H, int64_t Hk, int64_t T,
-                         int64_t D, int64_t q_sb, int64_t q_sh, int64_t q_st, const void *k,
-                         int64_t k_sb, int64_t k_sh, int64_t k_st, const void *v, int64_t v_sb,
-                         int64_t v_sh, int64_t v_st, int64_t L, int64_t window, int64_t sinks,
-                         const int64_t *lengths, float scale, void *out, int64_t o_sb,
-                         int64_t o_sh, int64_t o_st, void *workspace, size_t workspace_bytes,
-                         void *stream) {
+int mtp_window_attention(const mtp_window_args *p, void *stream) {
   WinArgs a{};
-  const int s = win_args(a, q, dtype, B, H, Hk, T, D, q_sb, q_sh, q_st, k, v, L, window, sinks,
-                         scale, out, o_sb, o_sh, o_st);
+  const int s = win_args(a, p);
   if (s < 0) return s;
-  if (L < T) return MTP_ERR_SHAPE;
+  if (p->L < p->T) return MTP_ERR_SHAPE;
   if (s > 0) return MTP_OK;
-  a.k_sb = k_sb, a.k_sh = k_sh, a.k_st = k_st;
-  a.v_sb = v_sb, a.v_sh = v_sh, a.v_st = v_st;
-  a.start_host = L - T;
-  a.lengths = lengths;
-  return win_launch(a, dtype, workspace, workspace_bytes, (hipStream_t)stream);
+  a.k_sb = p->k_st[0], a.k_sh = p->k_st[1], a.k_st = p->k_st[2];
+  a.v_sb = p->v_st[0], a.v_sh = p->v_st[1], a.v_st = p->v_st[2];
+  a.start_host = p->L - p->T;
+  a.lengths = p->lengths;
+  return win_launch(a, p->dtype, p->workspace, p->workspace_bytes, (hipStream_t)stream);
 }
 
-int mtp_paged_window_attention(const void *q, int dtype, int64_t B, int64_t H, int64_t Hk,
-                               int64_t T, int64_t D, int64_t q_sb, int64_t q_sh, int64_t q_st,
-                               const void *k_pages, const void *v_pages, int64_t num_pages,
-                               const int32_t *page_table, int64_t L, int64_t page_size,
-                               const int64_t *start_dev, int start_per_row, int64_t start_host,
-                               int64_t window, int64_t sinks, float scale, void *out, int64_t o_sb,
-                               int64_t o_sh, int64_t o_st, float *weights, void *workspace,
-                               size_t workspace_bytes, void *stream) {
+int mtp_paged_window_attention(const mtp_window_args *p, void *stream) {
   WinArgs a{};
-  const int s = win_args(a, q, dtype, B, H, Hk, T, D, q_sb, q_sh, q_st, k_pages, v_pages, L,
-                         window, sinks, scale, out, o_sb, o_sh, o_st);
+  const int s = win_args(a, p);
   if (s < 0) return s;
-  if (num_pages < 0 || num_pages > INT32_MAX || page_size <= 0 || page_size > INT32_MAX ||
-      (weights && B * Hk > 65535))
+  if (p->num_pages < 0 || p->num_pages > INT32_MAX || p->page_size <= 0 ||
+      p->page_size > INT32_MAX || (p->weights && p->B * p->Hk > 65535))
     return MTP_ERR_SHAPE;
   if (s > 0) return MTP_OK;
-  if (L > 0 && !page_table) return MTP_ERR_NULL;
-  a.k_st = D;
-  a.k_sh = page_size * D;
-  a.k_sb = Hk * a.k_sh;
-  a.p_sp = B * a.k_sb;
+  if (p->L > 0 && !p->page_table) return MTP_ERR_NULL;
+  a.k_st = p->D;
+  a.k_sh = p->page_size * p->D;
+  a.k_sb = p->Hk * a.k_sh;
+  a.p_sp = p->B * a.k_sb;
   a.v_sb = a.k_sb, a.v_sh = a.k_sh, a.v_st = a.k_st;
-  a.table = page_table;
-  a.ld_tab = L;
-  a.page_size = (int)page_size;
-  a.npages = (int)num_pages;
-  a.start_dev = start_dev;
-  a.start_per_row = start_per_row ? 1 : 0;
-  a.start_host = start_host;
-  a.weights = L > 0 ? weights : nullptr;
-  return win_launch(a, dtype, workspace, workspace_bytes, (hipStream_t)stream);
+  a.table = p->page_table;
+  a.ld_tab = p->L;
+  a.page_size = (int)p->page_size;
+  a.npages = (int)p->num_pages;
+  a.start_dev = p->start_dev;
+  a.start_per_row = p->start_per_row ? 1 : 0;
+  a.start_host = p->start_host;
+  a.weights = p->L > 0 ? p->weights : nullptr;
+  return win_launch(a, p->dtype, p->workspace, p->workspace_bytes, (hipStream_t)stream);
 }
 
 int mtp_kv_evict(const float *weights, const int64_t *lengths, int64_t B, int64_t Hk, int64_t L,

@@ -48,11 +48,8 @@ struct RopeArgs {
   float eps;
 };
 
-// sin and cos of position * inv_freq[i].
-__device__ __forceinline__ void rope_angle(const RopeArgs &a, int64_t pos, int i, float &s,
-                                           float &c) {
-  const double f = a.freq64 ? ((const double *)a.inv_freq)[i]
-                            : (double)((const float *)a.inv_freq)[i];
+// sin and cos of position * f.
+__device__ __forceinline__ void rope_angle(int64_t pos, double f, float &s, float &c) {
   const double turns = (double)pos * (f * 0.15915494309189533577);
   sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
 }
@@ -91,121 +88,173 @@ __device__ __forceinline__ u32x4 rope_pack(const float *f) {
 }
 
 // 16-byte form: rows of whole 16-byte chunks, at most LPR of them, every
-// pair's halves in whole chunks. Wave (token, part) takes the rows part *
-// RPI + i of the token, then every hs * RPI further on.
+// pair's halves in whole chunks. A token's rows come in steps of RPI: those of
+// its queries, then of its keys, then of its values; wave (token, part) takes
+// the steps part, part + hs, ...
 template <int DT, int LPR, bool INTER>
 __global__ void __launch_bounds__(256) rope_kernel(const RopeArgs a) {
   constexpr int VEC = 16 / dtype_bytes(DT);
   constexpr int RPI = 64 / LPR;
-  constexpr int U = 4;  // rows of a lane in flight
+  constexpr int U = 4;  // steps in flight
   const int lane = threadIdx.x & 63;
-  const int64_t wid = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t wid =
+      (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t tok = wid / a.hs;
   const int part = (int)(wid % a.hs);
   if (tok >= (int64_t)a.B * a.T) return;
   const int b = (int)(tok / a.T), t = (int)(tok % a.T);
-  const int c = lane % LPR, d0 = c * VEC;
+  const int sub = lane / LPR, c = lane % LPR, d0 = c * VEC;
   const bool on = d0 < a.D;
+  const int nq = (a.H + RPI - 1) / RPI, nk = (a.Hk + RPI - 1) / RPI;
+  const int steps = nq + nk + (a.v ? nk : 0);
+
+  const char *const qs = (const char *)a.q +
+      ((int64_t)b * a.q_sb + (int64_t)t * a.q_st + d0) * dtype_bytes(DT);
+  const char *const ks = (const char *)a.k +
+      ((int64_t)b * a.k_sb + (int64_t)t * a.k_st + d0) * dtype_bytes(DT);
+  const char *const vs = (const char *)a.v +
+      ((int64_t)b * a.v_sb + (int64_t)t * a.v_st + d0) * dtype_bytes(DT);
+  u32x4 w[U];
+  auto fetch = [&](int st) -> u32x4 {  // st is the same for the wave
+    u32x4 x = {0u, 0u, 0u, 0u};
+    if (st < nq) {
+      const int r = st * RPI + sub;
+      if (on && r < a.H) x = *(const u32x4 *)(qs + (int64_t)r * a.q_sh * dtype_bytes(DT));
+    } else if (st < steps) {
+      const bool key = st < nq + nk;
+      const int r = (st - nq - (key ? 0 : nk)) * RPI + sub;
+      if (on && r < a.Hk)
+        x = *(const u32x4 *)((key ? ks : vs) +
+                             (int64_t)r * (key ? a.k_sh : a.v_sh) * dtype_bytes(DT));
+    }
+    return x;
+  };
+  // the first rows are asked for before what their results need is computed
+#pragma unroll
+  for (int u = 0; u < U; ++u) w[u] = fetch(part + u * a.hs);
+
+  const int half = a.rot >> 1;
+  const bool rotated = on && d0 < a.rot;
+  const int hc = half / VEC;
+  const int mate = INTER || !rotated ? lane : (d0 < half ? lane + hc : lane - hc);
+  const int e0 = on ? d0 : 0, m0 = e0 + (mate - lane) * VEC;  // the partner's first element
+  // every load of the token before the first use of one: frequencies as raw
+  // bits, so that their conversion does not wait here
+  constexpr int NF = INTER ? VEC / 2 : VEC;
+  const int f0 = !rotated ? 0 : INTER ? d0 / 2 : (d0 < half ? d0 : d0 - half);
+  uint32_t flo[NF], fhi[NF];
+#pragma unroll
+  for (int i = 0; i < NF; ++i) flo[i] = fhi[i] = 0u;
+  if (a.rot > 0) {
+    if (a.freq64) {
+#pragma unroll
+      for (int i = 0; i < NF; ++i) {
+        const uint2 x = ((const uint2 *)a.inv_freq)[f0 + i];
+        flo[i] = x.x;
+        fhi[i] = x.y;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NF; ++i) flo[i] = ((const uint32_t *)a.inv_freq)[f0 + i];
+    }
+  }
+  // y = rs * (x * A + partner * B): A the gain times cos, B the partner's gain
+  // times -+ sin, for queries and for keys
+  float A[2][VEC], B[2][VEC];
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const float *const g = !a.norm ? nullptr : q == 0 ? a.wq : a.wk;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) A[q][i] = B[q][i] = 1.f;
+    if (g) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        A[q][i] = g[e0 + i];
+        B[q][i] = g[INTER ? e0 + (i ^ 1) : m0 + i];
+      }
+    }
+  }
   const int64_t start = a.start_dev ? a.start_dev[a.start_per_row ? b : 0] : a.start_host;
   const int64_t at = start + t;
   const int64_t pos = a.pos ? a.pos[(int64_t)b * a.pos_sb + t] : at;
   const int64_t slot = a.v ? rope_slot(a, b, at) : -1;
-  const int nqk = a.H + a.Hk, nr = nqk + (a.v ? a.Hk : 0);
-
-  // angles of the lane's elements (a pair shares one)
-  constexpr int NF = INTER ? VEC / 2 : VEC;
-  float cs[NF], sn[NF];
-  const int half = a.rot >> 1;
-  const bool rotated = d0 < a.rot;
-  const int f0 = INTER ? d0 / 2 : (d0 < half ? d0 : d0 - half);
 #pragma unroll
   for (int i = 0; i < NF; ++i) {
-    cs[i] = 1.f;
-    sn[i] = 0.f;
-    if (on && rotated) rope_angle(a, pos, f0 + i, sn[i], cs[i]);
-    if (!INTER && d0 < half) sn[i] = -sn[i];  // the first of a pair loses y_b sin t
+    float sn = 0.f, cs = 1.f;
+    if (rotated) {
+      const double f = a.freq64 ? __longlong_as_double((long long)fhi[i] << 32 | flo[i])
+                                : (double)__uint_as_float(flo[i]);
+      rope_angle(pos, f, sn, cs);
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      if constexpr (INTER) {
+        A[q][2 * i] *= cs;
+        A[q][2 * i + 1] *= cs;
+        B[q][2 * i] *= -sn;
+        B[q][2 * i + 1] *= sn;
+      } else {
+        A[q][i] *= cs;
+        B[q][i] *= d0 < half ? -sn : sn;
+      }
+    }
   }
-  const int hc = half / VEC;
-  const int mate = INTER || !rotated ? lane : (d0 < half ? lane + hc : lane - hc);
-  const int m0 = d0 + (mate - lane) * VEC;  // the partner's first element
   const float inv_d = 1.f / (float)a.D;
 
-  auto src_of = [&](int r) -> const char * {
-    int64_t off;
-    const char *p;
-    if (r < a.H) {
-      p = (const char *)a.q;
-      off = (int64_t)b * a.q_sb + (int64_t)r * a.q_sh + (int64_t)t * a.q_st;
-    } else if (r < nqk) {
-      p = (const char *)a.k;
-      off = (int64_t)b * a.k_sb + (int64_t)(r - a.H) * a.k_sh + (int64_t)t * a.k_st;
-    } else {
-      p = (const char *)a.v;
-      off = (int64_t)b * a.v_sb + (int64_t)(r - nqk) * a.v_sh + (int64_t)t * a.v_st;
+  auto turn = [&](u32x4 raw, const float(&ca)[VEC], const float(&cb)[VEC]) -> u32x4 {
+    float x[VEC], y[VEC];
+    rope_unpack<DT>(raw, x);
+    float rs = 1.f;
+    if (a.norm) {
+      float ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) ss = fmaf(x[i], x[i], ss);
+      rs = rsqrtf(sum_over_lanes<LPR>(ss) * inv_d + a.eps);
     }
-    return p + (off + d0) * dtype_bytes(DT);
-  };
-  auto dst_of = [&](int r) -> char * {
-    int64_t off;
-    char *p;
-    if (r < a.H) {
-      p = (char *)a.qo;
-      off = (int64_t)b * a.qo_sb + (int64_t)r * a.qo_sh + (int64_t)t * a.qo_st;
-    } else if (a.ko && r < nqk) {
-      p = (char *)a.ko;
-      off = (int64_t)b * a.ko_sb + (int64_t)(r - a.H) * a.ko_sh + (int64_t)t * a.ko_st;
+    if constexpr (INTER) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) y[i] = x[i ^ 1];
     } else {
-      if (slot < 0) return nullptr;
-      p = (char *)(r < nqk ? a.k_pages : a.v_pages);
-      off = slot + (int64_t)(r < nqk ? r - a.H : r - nqk) * a.p_sh;
+      u32x4 o;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = __shfl(raw[i], mate, 64);
+      rope_unpack<DT>(o, y);
     }
-    return p + (off + d0) * dtype_bytes(DT);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) y[i] = rs * fmaf(x[i], ca[i], y[i] * cb[i]);
+    return rope_pack<DT>(y);
   };
 
-  for (int r0 = part * RPI + lane / LPR; r0 - lane / LPR < nr; r0 += U * a.hs * RPI) {
-    u32x4 w[U];
+  for (int s0 = part; s0 < steps; s0 += U * a.hs) {
+    u32x4 x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = w[u];
+#pragma unroll
+    for (int u = 0; u < U; ++u) w[u] = fetch(s0 + (U + u) * a.hs);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int r = r0 + u * a.hs * RPI;
-      w[u] = u32x4{0u, 0u, 0u, 0u};
-      if (on && r < nr) w[u] = *(const u32x4 *)src_of(r);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int r = r0 + u * a.hs * RPI;
-      if (r - lane / LPR >= nr) break;  // wave-uniform
-      float x[VEC], y[VEC];
-      rope_unpack<DT>(w[u], x);
-      float rs = 1.f;
-      if (a.norm) {
-        float ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) ss = fmaf(x[i], x[i], ss);
-        rs = rsqrtf(sum_over_lanes<LPR>(ss) * inv_d + a.eps);
-      }
-      const float *const g = r < a.H ? a.wq : a.wk;
-      const bool gain = a.norm && g != nullptr;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) x[i] *= rs * (gain && on ? g[d0 + i] : 1.f);
-      if constexpr (INTER) {
-#pragma unroll
-        for (int i = 0; i < VEC; i += 2) {
-          y[i] = x[i] * cs[i / 2] - x[i + 1] * sn[i / 2];
-          y[i + 1] = x[i + 1] * cs[i / 2] + x[i] * sn[i / 2];
+      const int st = s0 + u * a.hs;
+      if (st < nq) {
+        const u32x4 y = turn(x[u], A[0], B[0]);
+        const int r = st * RPI + sub;
+        if (on && r < a.H)
+          *(u32x4 *)((char *)a.qo + ((int64_t)b * a.qo_sb + (int64_t)r * a.qo_sh +
+                                     (int64_t)t * a.qo_st + d0) * dtype_bytes(DT)) = y;
+      } else if (st < nq + nk) {
+        const u32x4 y = turn(x[u], A[1], B[1]);
+        const int r = (st - nq) * RPI + sub;
+        if (on && r < a.Hk) {
+          if (a.ko)
+            *(u32x4 *)((char *)a.ko + ((int64_t)b * a.ko_sb + (int64_t)r * a.ko_sh +
+                                       (int64_t)t * a.ko_st + d0) * dtype_bytes(DT)) = y;
+          else if (slot >= 0)
+            *(u32x4 *)((char *)a.k_pages + (slot + (int64_t)r * a.p_sh + d0) * dtype_bytes(DT)) = y;
         }
-      } else {
-        u32x4 o;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = __shfl(w[u][i], mate, 64);
-        rope_unpack<DT>(o, y);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float z = y[i] * (rs * (gain && on ? g[m0 + i] : 1.f));
-          y[i] = rotated ? x[i] * cs[i] + z * sn[i] : x[i];
-        }
+      } else if (st < steps) {
+        const int r = (st - nq - nk) * RPI + sub;
+        if (on && r < a.Hk && slot >= 0)
+          *(u32x4 *)((char *)a.v_pages + (slot + (int64_t)r * a.p_sh + d0) * dtype_bytes(DT)) = x[u];
       }
-      if (on && r < nr)
-        if (char *const p = dst_of(r)) *(u32x4 *)p = r < nqk ? rope_pack<DT>(y) : w[u];
     }
   }
 }
@@ -267,7 +316,8 @@ __global__ void __launch_bounds__(64) rope_generic_kernel(const RopeArgs a, int 
       const bool first = a.interleaved ? !(d & 1) : d < half;
       const int m = a.interleaved ? d ^ 1 : (first ? d + half : d - half);
       float s, c;
-      rope_angle(a, pos, i, s, c);
+      rope_angle(pos, a.freq64 ? ((const double *)a.inv_freq)[i]
+                               : (double)((const float *)a.inv_freq)[i], s, c);
       y = first ? y * c - s_y[m] * s : y * c + s_y[m] * s;
     }
     store_from_f32(dst, dt, dof + d, y);

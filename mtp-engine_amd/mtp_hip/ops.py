@@ -8,7 +8,6 @@ synchronising. Inputs must live on a HIP device.
 """
 from __future__ import annotations
 
-import functools
 import math
 from typing import Optional, Tuple
 
@@ -684,77 +683,100 @@ def batch_prefix_match(ids: torch.Tensor) -> torch.Tensor:
 
 
 # ---------------------------------------------------------------------------
-# Serving around the paged cache
-def _on_its_device(fn):
-    """The call runs with its first tensor's device as the current one: a
-    launch goes to the current device whatever its stream."""
-    @functools.wraps(fn)
-    def call(first, *args, **kwargs):
-        if first.is_cuda and first.get_device() != torch.cuda.current_device():
-            with torch.cuda.device(first.device):
-                return fn(first, *args, **kwargs)
-        return fn(first, *args, **kwargs)
-    return call
+# Serving around the paged cache. One token's call is a few microseconds on the
+# GPU, so the checks below read each tensor's attributes once.
+_current_device = getattr(torch._C, "_cuda_getDevice", lambda: -1)
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    return t if t.stride(-1) == 1 else t.contiguous()
+def _elsewhere(t: torch.Tensor) -> bool:
+    """t is on a HIP device that is not the current one: a launch goes to the
+    current device, whatever its stream."""
+    return t.is_cuda and t.get_device() != _current_device()
+
+
+def _same_device(first_name: str, first: torch.Tensor, **others) -> None:
+    d = first.get_device()
+    if d < 0:
+        _on_device(first_name, first)
+    for o in others.values():
+        if o is not None and o.get_device() != d:
+            _on_device(first_name, first, **others)
+
+
+def _i64(t: torch.Tensor) -> torch.Tensor:
+    t = t if t.is_contiguous() else t.contiguous()
+    return t if t.dtype is torch.int64 else t.to(torch.int64)
+
+
+def _rows(t: torch.Tensor):
+    """(t with d contiguous, its batch, head and token strides)"""
+    s = t.stride()
+    if s[3] != 1:
+        t = t.contiguous()
+        s = t.stride()
+    return t, s[0], s[1], s[2]
 
 
 def _start_arg(name: str, start, B: int):
     """(device tensor or None, per row, host value) of a start position: an
     int, or an int64 device tensor of one element (shared) or [B]."""
-    if torch.is_tensor(start):
-        dev = start.contiguous().to(torch.int64)
-        assert dev.numel() in (1, B), f"{name}: start must hold 1 or B positions"
-        return dev, int(dev.numel() == B and B > 1), 0
+    if isinstance(start, torch.Tensor):
+        start = _i64(start)
+        n = start.numel()
+        assert n == B or n == 1, f"{name}: start must hold 1 or B positions"
+        return start, int(n == B and B > 1), 0
     return None, 0, int(start)
 
 
 def _pages_arg(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
-               B: int, Hk: int, D: int, dtype) -> torch.Tensor:
-    """Checks pages [P, B, Hk, page_size, D] and the table [B, L]; the table
-    as int32."""
-    assert k_pages.dim() == 5 and k_pages.is_contiguous() and v_pages.is_contiguous() and \
-        v_pages.shape == k_pages.shape, \
-        f"{name}: pages must be contiguous [P, B, Hk, page_size, D], both alike"
-    assert (k_pages.shape[1], k_pages.shape[2], k_pages.shape[4]) == (B, Hk, D), \
-        f"{name}: pages {tuple(k_pages.shape)} do not match B={B}, Hk={Hk}, D={D}"
-    assert k_pages.dtype == dtype and v_pages.dtype == dtype, f"{name}: dtypes differ"
-    assert page_table.dim() == 2 and page_table.shape[0] == B, f"{name}: page_table [{B}, L]"
-    return _i32(page_table.contiguous())
+               B: int, D: int, dtype):
+    """Checks pages [P, B, Hk, page_size, D] and the table [B, L]; returns (the
+    table as int32, P, Hk, page_size, L)."""
+    shape = k_pages.shape
+    assert len(shape) == 5 and v_pages.shape == shape and k_pages.is_contiguous() and \
+        v_pages.is_contiguous(), f"{name}: pages must be contiguous [P, B, Hk, page_size, D], both alike"
+    P, _B, Hk, ps, _D = shape
+    assert _B == B and _D == D, f"{name}: pages {tuple(shape)} do not match B={B}, D={D}"
+    assert k_pages.dtype is dtype and v_pages.dtype is dtype, f"{name}: dtypes differ"
+    tshape = page_table.shape
+    assert len(tshape) == 2 and tshape[0] == B, f"{name}: page_table must be [{B}, L]"
+    if page_table.dtype is not torch.int32 or not page_table.is_contiguous():
+        page_table = _i32(page_table.contiguous())
+    return page_table, P, Hk, ps, tshape[1]
 
 
 def _rope_args(name: str, q, k, inv_freq, start, positions, q_weight, k_weight):
     assert q.dim() == 4 and k.dim() == 4, f"{name}: q [B, H, T, D], k [B, Hk, T, D]"
-    q, k = _rows(q), _rows(k)
     B, H, T, D = q.shape
-    assert (k.shape[0], k.shape[2], k.shape[3]) == (B, T, D), \
+    kB, Hk, kT, kD = k.shape
+    assert kB == B and kT == T and kD == D, \
         f"{name}: k must be [{B}, Hk, {T}, {D}], got {tuple(k.shape)}"
-    assert k.dtype == q.dtype, f"{name}: dtypes differ"
+    assert k.dtype is q.dtype, f"{name}: dtypes differ"
+    fdt = inv_freq.dtype
+    if fdt is not torch.float32 and fdt is not torch.float64:
+        raise TypeError(f"{name}: inv_freq must be float32 or float64, got {fdt}")
     inv_freq = inv_freq.contiguous()
-    if inv_freq.dtype not in (torch.float32, torch.float64):
-        raise TypeError(f"{name}: inv_freq must be float32 or float64, got {inv_freq.dtype}")
     rot = 2 * inv_freq.numel()
     assert inv_freq.dim() == 1 and rot <= D, f"{name}: inv_freq holds at most D / 2 frequencies"
     pos_sb = 0
     if positions is not None:
-        assert positions.dim() in (1, 2) and positions.shape[-1] == T and \
-            (positions.dim() == 1 or positions.shape[0] in (1, B)), \
+        pd = positions.dim()
+        assert pd in (1, 2) and positions.shape[-1] == T and \
+            (pd == 1 or positions.shape[0] in (1, B)), \
             f"{name}: positions must be [{T}], [1, {T}] or [{B}, {T}]"
-        positions = positions.contiguous().to(torch.int64)
-        pos_sb = T if positions.dim() == 2 and positions.shape[0] == B else 0
-    ws = []
-    for w in (q_weight, k_weight):
-        if w is not None:
-            w = _f32(w.contiguous())
-            assert w.numel() == D, f"{name}: a norm weight has {w.numel()} != {D}"
-        ws.append(w)
+        positions = _i64(positions)
+        pos_sb = T if pd == 2 and positions.shape[0] == B else 0
+    if q_weight is not None:
+        q_weight = _f32(q_weight.contiguous())
+        assert q_weight.numel() == D, f"{name}: q_weight has {q_weight.numel()} != {D}"
+    if k_weight is not None:
+        k_weight = _f32(k_weight.contiguous())
+        assert k_weight.numel() == D, f"{name}: k_weight has {k_weight.numel()} != {D}"
     start_dev, per_row, start_host = _start_arg(name, start, B)
-    return q, k, inv_freq, rot, positions, pos_sb, ws[0], ws[1], start_dev, per_row, start_host
+    return (B, H, Hk, T, D, inv_freq, int(fdt is torch.float64), rot, positions, pos_sb, q_weight,
+            k_weight, start_dev, per_row, start_host)
 
 
-@_on_its_device
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor, start=0,
                  positions: Optional[torch.Tensor] = None,
                  q_weight: Optional[torch.Tensor] = None,
@@ -769,23 +791,31 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor, start
     paged_kv_write. The outputs keep the inputs' order of dimensions in
     memory."""
     name = "qk_norm_rope"
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return qk_norm_rope(q, k, inv_freq, start, positions, q_weight, k_weight, eps, norm,
+                                interleaved)
     lib = _lib.load()
-    q, k, f, rot, positions, pos_sb, wq, wk, start_dev, per_row, start_host = _rope_args(
-        name, q, k, inv_freq, start, positions, q_weight, k_weight)
-    _on_device("q", q, k=k, inv_freq=f, positions=positions, q_weight=wq, k_weight=wk,
-               start=start_dev)
-    B, H, T, D = q.shape
+    (B, H, Hk, T, D, f, f64, rot, positions, pos_sb, wq, wk, start_dev, per_row,
+     start_host) = _rope_args(name, q, k, inv_freq, start, positions, q_weight, k_weight)
+    _same_device("q", q, k=k, inv_freq=f, positions=positions, q_weight=wq, k_weight=wk,
+                 start=start_dev)
+    q, q0, q1, q2 = _rows(q)
+    k, k0, k1, k2 = _rows(k)
     qo, ko = torch.empty_like(q), torch.empty_like(k)
-    s = lib.mtp_qk_norm_rope(
-        ptr(q), ptr(k), code(q.dtype), B, T, H, k.shape[1], D, *q.stride()[:3], *k.stride()[:3],
-        ptr(f), int(f.dtype is torch.float64), rot, int(bool(interleaved)), int(bool(norm)),
-        ptr(wq), ptr(wk), float(eps), ptr(positions), pos_sb, ptr(start_dev), per_row, start_host,
-        ptr(qo), *qo.stride()[:3], ptr(ko), *ko.stride()[:3], _lib.stream_handle(q.device))
-    check(s, name)
+    o0, o1, o2, _ = qo.stride()
+    p0, p1, p2, _ = ko.stride()
+    args = _lib.ROPE_ARGS.pack(
+        q.data_ptr(), k.data_ptr(), 0, qo.data_ptr(), ko.data_ptr(), 0, 0, 0, f.data_ptr(),
+        ptr(wq) or 0, ptr(wk) or 0, ptr(positions) or 0, ptr(start_dev) or 0, B, T, H, Hk, D,
+        q0, q1, q2, k0, k1, k2, 0, 0, 0, o0, o1, o2, p0, p1, p2, rot, pos_sb, start_host, 0, 1, 0,
+        eps, code(q.dtype), f64, bool(interleaved), bool(norm), per_row)
+    s = lib.mtp_qk_norm_rope(args, _lib.stream_handle(q.device))
+    if s:
+        check(s, name)
     return qo, ko
 
 
-@_on_its_device
 def qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, inv_freq: torch.Tensor,
                        k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
                        start, positions: Optional[torch.Tensor] = None,
@@ -799,26 +829,34 @@ def qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, inv_fr
     page_size, D] in q's dtype; positions outside the table and pages outside
     the pool are skipped."""
     name = "qk_norm_rope_write"
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return qk_norm_rope_write(q, k, v, inv_freq, k_pages, v_pages, page_table, start,
+                                      positions, q_weight, k_weight, eps, norm, interleaved)
     lib = _lib.load()
-    q, k, f, rot, positions, pos_sb, wq, wk, start_dev, per_row, start_host = _rope_args(
-        name, q, k, inv_freq, start, positions, q_weight, k_weight)
-    v = _rows(v)
-    assert v.shape == k.shape, f"{name}: v must be shaped like k, got {tuple(v.shape)}"
-    assert v.dtype == q.dtype, f"{name}: dtypes differ"
-    B, H, T, D = q.shape
-    Hk = k.shape[1]
-    page_table = _pages_arg(name, k_pages, v_pages, page_table, B, Hk, D, q.dtype)
-    _on_device("q", q, k=k, v=v, inv_freq=f, positions=positions, q_weight=wq, k_weight=wk,
-               start=start_dev, k_pages=k_pages, v_pages=v_pages, page_table=page_table)
+    (B, H, Hk, T, D, f, f64, rot, positions, pos_sb, wq, wk, start_dev, per_row,
+     start_host) = _rope_args(name, q, k, inv_freq, start, positions, q_weight, k_weight)
+    dt = q.dtype
+    assert v.shape == k.shape and v.dtype is dt, \
+        f"{name}: v must be like k, got {v.dtype} {tuple(v.shape)}"
+    page_table, P, pH, ps, L = _pages_arg(name, k_pages, v_pages, page_table, B, D, dt)
+    assert pH == Hk, f"{name}: pages of {pH} heads for {Hk}"
+    _same_device("q", q, k=k, v=v, inv_freq=f, positions=positions, q_weight=wq, k_weight=wk,
+                 start=start_dev, k_pages=k_pages, v_pages=v_pages, page_table=page_table)
+    q, q0, q1, q2 = _rows(q)
+    k, k0, k1, k2 = _rows(k)
+    v, v0, v1, v2 = _rows(v)
     qo = torch.empty_like(q)
-    s = lib.mtp_qk_norm_rope_write(
-        ptr(q), ptr(k), ptr(v), code(q.dtype), B, T, H, Hk, D, *q.stride()[:3], *k.stride()[:3],
-        *v.stride()[:3], ptr(f), int(f.dtype is torch.float64), rot, int(bool(interleaved)),
-        int(bool(norm)), ptr(wq), ptr(wk), float(eps), ptr(positions), pos_sb, ptr(start_dev),
-        per_row, start_host, ptr(qo), *qo.stride()[:3], ptr(k_pages), ptr(v_pages),
-        k_pages.shape[0], k_pages.shape[3], ptr(page_table), page_table.shape[1],
-        _lib.stream_handle(q.device))
-    check(s, name)
+    o0, o1, o2, _ = qo.stride()
+    args = _lib.ROPE_ARGS.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), qo.data_ptr(), 0, k_pages.data_ptr(),
+        v_pages.data_ptr(), page_table.data_ptr(), f.data_ptr(), ptr(wq) or 0, ptr(wk) or 0,
+        ptr(positions) or 0, ptr(start_dev) or 0, B, T, H, Hk, D, q0, q1, q2, k0, k1, k2, v0, v1,
+        v2, o0, o1, o2, 0, 0, 0, rot, pos_sb, start_host, P, ps, L, eps, code(dt), f64,
+        bool(interleaved), bool(norm), per_row)
+    s = lib.mtp_qk_norm_rope_write(args, _lib.stream_handle(q.device))
+    if s:
+        check(s, name)
     return qo
 
 
@@ -831,7 +869,22 @@ def _window_arg(name: str, window, sinks) -> Tuple[int, int]:
     return (-1 if window is None else min(int(window), 1 << 40)), min(int(sinks), 1 << 40)
 
 
-@_on_its_device
+def _window_call(name: str, fn, pack, q: torch.Tensor, sizes, paged: int, weights: int) -> None:
+    """Runs fn(pack(workspace, bytes)) with the stream's workspace as it is, and
+    only where that is too small (nothing has run then) asks for its size."""
+    idx = q.get_device()
+    stream = _lib.raw_stream(idx)
+    ws = _lib.current_workspace(idx, stream)
+    s = fn(pack(ws.data_ptr() if ws is not None else 0, ws.numel() if ws is not None else 0),
+           stream)
+    if s == _lib.ERR_WORKSPACE:
+        n = _lib.load().mtp_window_attention_workspace_bytes(code(q.dtype), *sizes, paged, weights)
+        at, stream = _lib.scratch(q, n)
+        s = fn(pack(at or 0, n), stream)
+    if s:
+        check(s, name)
+
+
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                      window: Optional[int] = None, sinks: int = 0,
                      lengths: Optional[torch.Tensor] = None,
@@ -844,36 +897,43 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     contiguous; lengths [B]: positions from lengths[b] on are padding (keys
     that nobody sees, rows of zeros). A row that sees no key is zero."""
     name = "window_attention"
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return window_attention(q, k, v, window, sinks, lengths, scale)
     lib = _lib.load()
     assert q.dim() == 4 and k.dim() == 4 and v.shape == k.shape, \
         f"{name}: q [B, H, T, D], k / v [B, Hk, L, D]"
-    q, k, v = _rows(q), _rows(k), _rows(v)
     B, H, T, D = q.shape
     _B, Hk, L, _D = k.shape
-    assert (_B, _D) == (B, D), f"{name}: k / v must be [{B}, Hk, L, {D}], got {tuple(k.shape)}"
+    assert _B == B and _D == D, f"{name}: k / v must be [{B}, Hk, L, {D}], got {tuple(k.shape)}"
     assert Hk > 0 and H % Hk == 0, f"{name}: {H} query heads over {Hk} key heads"
     assert T <= L, f"{name}: {T} queries but only {L} keys"
-    assert k.dtype == q.dtype and v.dtype == q.dtype, f"{name}: dtypes differ"
+    dt = q.dtype
+    assert k.dtype is dt and v.dtype is dt, f"{name}: dtypes differ"
     win, sinks = _window_arg(name, window, sinks)
     if lengths is not None:
-        lengths = lengths.contiguous().to(torch.int64)
+        lengths = _i64(lengths)
         assert tuple(lengths.shape) == (B,), f"{name}: lengths must be [{B}]"
-    _on_device("q", q, k=k, v=v, lengths=lengths)
+    _same_device("q", q, k=k, v=v, lengths=lengths)
+    q, q0, q1, q2 = _rows(q)
+    k, k0, k1, k2 = _rows(k)
+    v, v0, v1, v2 = _rows(v)
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     out = torch.empty_like(q)
-    dt = code(q.dtype)
-    nbytes = lib.mtp_window_attention_workspace_bytes(dt, B, H, Hk, T, D, L, win, sinks, 0, 0)
-    ws, stream = _lib.scratch(q, nbytes)
-    s = lib.mtp_window_attention(
-        ptr(q), dt, B, H, Hk, T, D, *q.stride()[:3], ptr(k), *k.stride()[:3], ptr(v),
-        *v.stride()[:3], L, win, sinks, ptr(lengths), float(scale), ptr(out), *out.stride()[:3],
-        ws, nbytes, stream)
-    check(s, name)
+    o0, o1, o2, _ = out.stride()
+    qp, kp, vp, op, lp, cd = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                              ptr(lengths) or 0, code(dt))
+
+    def pack(ws, nbytes):
+        return _lib.WINDOW_ARGS.pack(qp, kp, vp, op, 0, 0, lp, 0, ws, nbytes, B, H, Hk, T, D, L,
+                                     q0, q1, q2, k0, k1, k2, v0, v1, v2, o0, o1, o2, win, sinks, 0,
+                                     0, 1, scale, cd, 0)
+
+    _window_call(name, lib.mtp_window_attention, pack, q, (B, H, Hk, T, D, L, win, sinks), 0, 0)
     return out
 
 
-@_on_its_device
 def paged_window_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                            page_table: torch.Tensor, page_size: int, start,
                            window: Optional[int] = None, sinks: int = 0,
@@ -888,38 +948,45 @@ def paged_window_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     received, summed over the queries and over the heads of its group, is
     added in place."""
     name = "paged_window_attention"
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return paged_window_attention(q, k_pages, v_pages, page_table, page_size, start,
+                                          window, sinks, scale, weights)
     lib = _lib.load()
     assert q.dim() == 4, f"{name}: q [B, H, T, D]"
-    q = _rows(q)
     B, H, T, D = q.shape
-    Hk = k_pages.shape[2] if k_pages.dim() == 5 else 0
-    page_table = _pages_arg(name, k_pages, v_pages, page_table, B, Hk, D, q.dtype)
-    assert k_pages.shape[3] == page_size, f"{name}: pages hold {k_pages.shape[3]} slots"
+    dt = q.dtype
+    page_table, P, Hk, ps, L = _pages_arg(name, k_pages, v_pages, page_table, B, D, dt)
+    assert ps == page_size, f"{name}: pages hold {ps} slots, not {page_size}"
     assert Hk > 0 and H % Hk == 0, f"{name}: {H} query heads over {Hk} key heads"
-    L = page_table.shape[1]
     win, sinks = _window_arg(name, window, sinks)
     start_dev, per_row, start_host = _start_arg(name, start, B)
+    wp = 0
     if weights is not None:
-        assert tuple(weights.shape) == (B, Hk, L) and weights.dtype == torch.float32 and \
+        assert weights.shape == (B, Hk, L) and weights.dtype is torch.float32 and \
             weights.is_contiguous(), f"{name}: weights must be contiguous float32 [{B}, {Hk}, {L}]"
-    _on_device("q", q, k_pages=k_pages, v_pages=v_pages, page_table=page_table, start=start_dev,
-               weights=weights)
+        wp = weights.data_ptr()
+    _same_device("q", q, k_pages=k_pages, v_pages=v_pages, page_table=page_table, start=start_dev,
+                 weights=weights)
+    q, q0, q1, q2 = _rows(q)
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     out = torch.empty_like(q)
-    dt = code(q.dtype)
-    nbytes = lib.mtp_window_attention_workspace_bytes(dt, B, H, Hk, T, D, L, win, sinks, 1,
-                                                      int(weights is not None))
-    ws, stream = _lib.scratch(q, nbytes)
-    s = lib.mtp_paged_window_attention(
-        ptr(q), dt, B, H, Hk, T, D, *q.stride()[:3], ptr(k_pages), ptr(v_pages), k_pages.shape[0],
-        ptr(page_table), L, int(page_size), ptr(start_dev), per_row, start_host, win, sinks,
-        float(scale), ptr(out), *out.stride()[:3], ptr(weights), ws, nbytes, stream)
-    check(s, name)
+    o0, o1, o2, _ = out.stride()
+    qp, kp, vp, op, tp, sp, cd = (q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                                  out.data_ptr(), page_table.data_ptr(), ptr(start_dev) or 0,
+                                  code(dt))
+
+    def pack(ws, nbytes):
+        return _lib.WINDOW_ARGS.pack(qp, kp, vp, op, tp, sp, 0, wp, ws, nbytes, B, H, Hk, T, D, L,
+                                     q0, q1, q2, 0, 0, 0, 0, 0, 0, o0, o1, o2, win, sinks,
+                                     start_host, P, ps, scale, cd, per_row)
+
+    _window_call(name, lib.mtp_paged_window_attention, pack, q, (B, H, Hk, T, D, L, win, sinks), 1,
+                 int(wp != 0))
     return out
 
 
-@_on_its_device
 def kv_evict(weights: torch.Tensor, lengths: torch.Tensor, k_pages: torch.Tensor,
              v_pages: torch.Tensor, page_table: torch.Tensor, out_table: torch.Tensor,
              sinks: int = 0, recent: int = 0):
@@ -935,35 +1002,42 @@ def kv_evict(weights: torch.Tensor, lengths: torch.Tensor, k_pages: torch.Tensor
     pages [P, B, Hk, page_size, D] of any dtype; the copied keys keep the
     rotation they were written with."""
     name = "kv_evict"
+    if _elsewhere(weights):
+        with torch.cuda.device(weights.device):
+            return kv_evict(weights, lengths, k_pages, v_pages, page_table, out_table, sinks,
+                            recent)
     lib = _lib.load()
-    assert weights.dim() == 3 and weights.dtype == torch.float32, f"{name}: weights fp32 [B, Hk, L]"
+    assert weights.dim() == 3 and weights.dtype is torch.float32, \
+        f"{name}: weights must be float32 [B, Hk, L]"
     weights = weights.contiguous()
     B, Hk, L = weights.shape
-    assert Hk > 0, f"{name}: no key heads"
     D = k_pages.shape[-1]
-    assert k_pages.dtype == v_pages.dtype, f"{name}: dtypes differ"
-    page_table = _pages_arg(name, k_pages, v_pages, page_table, B, Hk, D, k_pages.dtype)
-    assert page_table.shape[1] == L, f"{name}: page_table has {page_table.shape[1]} != {L} positions"
-    assert out_table.dim() == 2 and out_table.shape[0] == B and out_table.shape[1] > 0, \
+    page_table, P, pH, ps, _L = _pages_arg(name, k_pages, v_pages, page_table, B, D, k_pages.dtype)
+    assert pH == Hk and Hk > 0, f"{name}: pages of {pH} heads for weights of {Hk}"
+    assert _L == L, f"{name}: page_table has {_L} != {L} positions"
+    oshape = out_table.shape
+    assert len(oshape) == 2 and oshape[0] == B and oshape[1] > 0, \
         f"{name}: out_table must be [{B}, keep]"
-    out_table = _i32(out_table.contiguous())
-    if out_table.numel() and out_table.data_ptr() == page_table.data_ptr():
+    if out_table.dtype is not torch.int32 or not out_table.is_contiguous():
+        out_table = _i32(out_table.contiguous())
+    if B and out_table.data_ptr() == page_table.data_ptr():
         raise ValueError(f"{name}: out_table is page_table: rows cannot move onto themselves")
-    keep = out_table.shape[1]
+    keep = oshape[1]
     sinks, recent = int(sinks), int(recent)
     if sinks < 0 or recent < 0 or sinks + recent > keep:
         raise ValueError(f"{name}: sinks {sinks} and recent {recent} must fit in keep {keep}")
-    lengths = lengths.contiguous().to(torch.int64)
-    assert tuple(lengths.shape) == (B,), f"{name}: lengths must be [{B}]"
-    _on_device("weights", weights, lengths=lengths, k_pages=k_pages, v_pages=v_pages,
-               page_table=page_table, out_table=out_table)
-    dev = weights.device
-    kept = torch.empty((B, Hk, keep), dtype=torch.int32, device=dev)
-    w = torch.empty((B, Hk, keep), dtype=torch.float32, device=dev)
-    n = torch.empty((B,), dtype=torch.int64, device=dev)
-    s = lib.mtp_kv_evict(ptr(weights), ptr(lengths), B, Hk, L, keep, sinks, recent, ptr(k_pages),
-                         ptr(v_pages), k_pages.shape[0], k_pages.shape[3],
-                         D * k_pages.element_size(), ptr(page_table), ptr(out_table), ptr(kept),
-                         ptr(w), ptr(n), _lib.stream_handle(dev))
-    check(s, name)
+    lengths = _i64(lengths)
+    assert lengths.dim() == 1 and lengths.shape[0] == B, f"{name}: lengths must be [{B}]"
+    _same_device("weights", weights, lengths=lengths, k_pages=k_pages, v_pages=v_pages,
+                 page_table=page_table, out_table=out_table)
+    kept = out_table.new_empty((B, Hk, keep))
+    w = weights.new_empty((B, Hk, keep))
+    n = torch.empty_like(lengths)
+    s = lib.mtp_kv_evict(weights.data_ptr(), lengths.data_ptr(), B, Hk, L, keep, sinks, recent,
+                         k_pages.data_ptr(), v_pages.data_ptr(), P, ps,
+                         D * k_pages.element_size(), page_table.data_ptr(), out_table.data_ptr(),
+                         kept.data_ptr(), w.data_ptr(), n.data_ptr(),
+                         _lib.stream_handle(weights.device))
+    if s:
+        check(s, name)
     return kept, w, n

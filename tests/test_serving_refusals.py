@@ -121,56 +121,60 @@ X = 4096  # never dereferenced: every call below returns before any HIP call
 STR = (64, 64, 64)
 
 
+def rope_pack(q=X, k=X, v=X, qo=X, ko=X, kp=X, vp=X, tab=X, f=X, b=1, t=2, h=2, hk=1, d=64, rot=64,
+              np_=4, ps=16, ld=8, dt=_lib.BF16):
+    z = [x or 0 for x in (q, k, v, qo, ko, kp, vp, tab, f)]
+    return _lib.ROPE_ARGS.pack(*z, 0, 0, 0, 0, b, t, h, hk, d, *STR, *STR, *STR, *STR, *STR, rot, 0,
+                               0, np_, ps, ld, 1e-6, dt, 0, 0, 1, 0)
+
+
 def test_rope_abi(lib):
-    def call(q=X, k=X, dt=_lib.BF16, b=1, t=2, h=2, hk=1, d=64, f=X, rot=64, qo=X, ko=X):
-        return lib.mtp_qk_norm_rope(q, k, dt, b, t, h, hk, d, *STR, *STR, f, 0, rot, 0, 1, None,
-                                    None, 1e-6, None, 0, None, 0, 0, qo, *STR, ko, *STR, None)
-
-    def write(v=X, kp=X, vp=X, np_=4, ps=16, tab=X, ld=8, b=1):
-        return lib.mtp_qk_norm_rope_write(X, X, v, _lib.BF16, b, 2, 2, 1, 64, *STR, *STR, *STR, X,
-                                          0, 64, 0, 1, None, None, 1e-6, None, 0, None, 0, 0, X,
-                                          *STR, kp, vp, np_, ps, tab, ld, None)
-
-    assert call(dt=_lib.FP8E4M3) == _lib.ERR_DTYPE
-    for kw in (dict(d=0), dict(d=5000), dict(rot=63), dict(rot=66), dict(rot=-2), dict(b=-1),
-               dict(h=70000)):
-        assert call(**kw) == _lib.ERR_SHAPE, kw
-    for kw in (dict(q=None), dict(k=None), dict(f=None), dict(qo=None), dict(ko=None)):
-        assert call(**kw) == _lib.ERR_NULL, kw
-    assert call(b=0, q=None, k=None) == _lib.OK and call(t=0) == _lib.OK
-    for kw in (dict(v=None), dict(kp=None), dict(vp=None), dict(tab=None)):
-        assert write(**kw) == _lib.ERR_NULL, kw
-    for kw in (dict(np_=-1), dict(ps=0), dict(ld=-1)):
-        assert write(**kw) == _lib.ERR_SHAPE, kw
-    assert write(b=0) == _lib.OK
+    for fn, write in ((lib.mtp_qk_norm_rope, False), (lib.mtp_qk_norm_rope_write, True)):
+        def call(**kw):
+            return fn(rope_pack(**kw), None)
+        assert fn(None, None) == _lib.ERR_NULL
+        assert call(dt=_lib.FP8E4M3) == _lib.ERR_DTYPE
+        for kw in (dict(d=0), dict(d=5000), dict(rot=63), dict(rot=66), dict(rot=-2), dict(b=-1),
+                   dict(h=70000)):
+            assert call(**kw) == _lib.ERR_SHAPE, kw
+        nulls = [dict(q=None), dict(k=None), dict(f=None), dict(qo=None)]
+        nulls += [dict(v=None), dict(kp=None), dict(vp=None), dict(tab=None)] if write else \
+            [dict(ko=None)]
+        for kw in nulls:
+            assert call(**kw) == _lib.ERR_NULL, kw
+        if write:
+            for kw in (dict(np_=-1), dict(ps=0), dict(ld=-1)):
+                assert call(**kw) == _lib.ERR_SHAPE, kw
+        assert call(b=0, q=None, k=None) == _lib.OK and call(t=0) == _lib.OK
 
 
 def test_window_attention_abi(lib):
-    def dense(q=X, dt=_lib.BF16, b=1, h=2, hk=1, t=2, d=64, k=X, v=X, l_=8, w=-1, s=0, o=X):
-        return lib.mtp_window_attention(q, dt, b, h, hk, t, d, *STR, k, *STR, v, *STR, l_, w, s,
-                                        None, 1.0, o, *STR, None, 0, None)
+    def pack(q=X, k=X, v=X, o=X, tab=X, weights=None, ws=None, nb=0, b=1, h=2, hk=1, t=2, d=64,
+             l_=8, w=-1, s=0, np_=4, ps=16, dt=_lib.BF16):
+        z = [x or 0 for x in (q, k, v, o, tab, None, None, weights, ws)]
+        return _lib.WINDOW_ARGS.pack(*z, nb, b, h, hk, t, d, l_, *STR, *STR, *STR, *STR, w, s, 0,
+                                     np_, ps, 1.0, dt, 0)
 
-    def paged(tab=X, np_=4, ps=16, weights=None, ws=None, nb=0, t=2, b=1, l_=8):
-        return lib.mtp_paged_window_attention(X, _lib.BF16, b, 2, 1, t, 64, *STR, X, X, np_, tab,
-                                              l_, ps, None, 0, 0, -1, 0, 1.0, X, *STR, weights, ws,
-                                              nb, None)
-
-    assert dense(dt=_lib.I32) == _lib.ERR_DTYPE
-    for kw in (dict(h=3, hk=2), dict(hk=0), dict(d=0), dict(d=1025), dict(t=9), dict(l_=1 << 30),
-               dict(b=-1)):
-        assert dense(**kw) == _lib.ERR_SHAPE, kw
-    for kw in (dict(w=0), dict(w=-2), dict(s=-1)):
-        assert dense(**kw) == _lib.ERR_ARG, kw
-    for kw in (dict(q=None), dict(k=None), dict(v=None), dict(o=None)):
-        assert dense(**kw) == _lib.ERR_NULL, kw
-    assert dense(t=0, l_=0, k=None, v=None) == _lib.OK and dense(b=0) == _lib.OK
-    assert paged(tab=None) == _lib.ERR_NULL
-    for kw in (dict(np_=-1), dict(ps=0), dict(l_=-1)):
-        assert paged(**kw) == _lib.ERR_SHAPE, kw
-    assert paged(b=0) == _lib.OK and paged(t=0) == _lib.OK
+    for fn, paged in ((lib.mtp_window_attention, False), (lib.mtp_paged_window_attention, True)):
+        def call(**kw):
+            return fn(pack(**kw), None)
+        assert fn(None, None) == _lib.ERR_NULL
+        assert call(dt=_lib.I32) == _lib.ERR_DTYPE
+        for kw in (dict(h=3, hk=2), dict(hk=0), dict(d=0), dict(d=1025), dict(l_=1 << 30),
+                   dict(b=-1), dict(np_=-1) if paged else dict(t=9),
+                   dict(ps=0) if paged else dict(t=-1), dict(l_=-1)):
+            assert call(**kw) == _lib.ERR_SHAPE, kw
+        for kw in (dict(w=0), dict(w=-2), dict(s=-1)):
+            assert call(**kw) == _lib.ERR_ARG, kw
+        for kw in (dict(q=None), dict(k=None), dict(v=None), dict(o=None),
+                   dict(tab=None) if paged else dict(q=None)):
+            assert call(**kw) == _lib.ERR_NULL, kw
+        assert call(t=0, l_=0, k=None, v=None) == _lib.OK and call(b=0) == _lib.OK
     # weights keep the scores in the workspace
     need = lib.mtp_window_attention_workspace_bytes(_lib.BF16, 1, 2, 1, 2, 64, 8, -1, 0, 1, 1)
-    assert need > 0 and paged(weights=X, ws=X, nb=need - 1) == _lib.ERR_WORKSPACE
+    assert need > 0
+    assert lib.mtp_paged_window_attention(pack(weights=X, ws=X, nb=need - 1), None) == \
+        _lib.ERR_WORKSPACE
     assert lib.mtp_window_attention_workspace_bytes(_lib.BF16, 0, 2, 1, 2, 64, 8, -1, 0, 1, 1) == 0
     # a window bounds the scores kept, not the table's width
     wide = lib.mtp_window_attention_workspace_bytes(_lib.BF16, 1, 2, 1, 1, 64, 1 << 20, 64, 4, 1, 1)
