@@ -126,9 +126,10 @@ int rope_args(RopeArgs &a, const mtp_rope_args *p) {
 // ---- windowed attention
 struct WinPlan {
   int rt = 0;              // split kernel: row tiles of a block; 0: one wave per row
+  int nw = 4;              // its waves
   int rblocks = 1, nchunks = 1;
   int64_t ld_sc = 0;       // scores (with weights)
-  size_t sc_off = 0, ml_off = 0, part_off = 0, pml_off = 0, total = 0;
+  size_t sc_off = 0, part_off = 0, pml_off = 0, total = 0;
 };
 
 // Keys that t queries can see of a sequence at most.
@@ -150,31 +151,43 @@ WinPlan win_plan(int dt, int64_t B, int64_t H, int64_t Hk, int64_t T, int64_t D,
   if (B <= 0 || H <= 0 || Hk <= 0 || H % Hk != 0 || T <= 0 || L <= 0) return p;
   const int64_t rows = H / Hk * T, units = B * Hk;
   size_t at = kCounterBytes;
-  if (win_split_pick(dt, (int)std::min<int64_t>(D, 1 << 20), 1, false)) {
+  if (win_split_pick(dt, (int)std::min<int64_t>(D, 1 << 20), 1, false, 4)) {
     p.rt = rows > 16 ? 2 : 1;
     const int64_t rp = 16 * p.rt;
     p.rblocks = (int)((rows + rp - 1) / rp);
     const int64_t most = win_most(std::min(T, (rp - 1) / (H / Hk) + 2), L, window, sinks);
-    const int64_t step = (int64_t)kWinSplitWaves * win_split_keys((int)D * dtype_bytes(dt));
-    const int64_t room = 2 * (int64_t)device_cus() / (units * p.rblocks);
-    p.nchunks = (int)std::max<int64_t>(1, std::min(room, most / (2 * step)));
+    const int64_t wgs = units * p.rblocks, sk = win_split_keys((int)D * dtype_bytes(dt));
+    // eight waves, a workgroup a CU, where that many workgroups suffice (chunks
+    // of a step for every wave); else four, so that two of them share a CU
+    p.nw = wgs <= device_cus() ? 8 : 4;
+    const int64_t room = 8 / p.nw * (int64_t)device_cus() / wgs;
+    p.nchunks = (int)std::max<int64_t>(1, std::min(room, most / (8 * sk)));
+    const int64_t parts = wgs * p.nchunks * rp;
     if (p.nchunks > 1) {
-      const int64_t parts = units * p.rblocks * p.nchunks * rp;
       p.part_off = at;
       at += align_up((size_t)parts * (size_t)D * 4, 256);
-      p.pml_off = at;
-      at += align_up((size_t)parts * 8, 256);
     }
+    if (p.nchunks > 1 || weights) {
+      p.pml_off = at;
+      at += align_up((size_t)std::max(parts, B * H * T) * 8, 256);
+    }
+  } else if (weights) {
+    p.pml_off = at;
+    at += align_up((size_t)(B * H * T) * 8, 256);
   }
   if (weights) {
     p.ld_sc = win_most(T, L, window, sinks);
     p.sc_off = at;
     at += align_up((size_t)(B * H * T) * (size_t)p.ld_sc * 4, 256);
-    p.ml_off = at;
-    at += align_up((size_t)(B * H * T) * 8, 256);
   }
   p.total = at > kCounterBytes ? at : 0;
   return p;
+}
+
+// The weights alone, after the kernel that takes a wave per row.
+__global__ void __launch_bounds__(256) win_weights_kernel(const WinArgs a) {
+  __shared__ float s_a[256], s_b[256];
+  win_weights(a, blockIdx.y, blockIdx.x, s_a, s_b);
 }
 
 template <bool PAGED>
@@ -196,8 +209,9 @@ int win_launch(WinArgs &a, int dt, void *workspace, size_t workspace_bytes, hipS
   if (a.weights) {
     a.scores = (float *)(w8 + p.sc_off);
     a.ld_sc = p.ld_sc;
-    a.ml = (float *)(w8 + p.ml_off);
   }
+  a.part = (float *)(w8 + p.part_off);
+  a.pml = (float *)(w8 + p.pml_off);
   const int64_t e = 16 / dtype_bytes(dt);
   const bool whole = aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.out) &&
                      mult({a.q_sb, a.q_sh, a.q_st, a.k_sb, a.k_sh, a.k_st, a.v_sb, a.v_sh, a.v_st,
@@ -215,27 +229,34 @@ int win_launch(WinArgs &a, int dt, void *workspace, size_t workspace_bytes, hipS
     a.rblocks = (int)pblocks;
     hipLaunchKernelGGL(prompt, dim3((unsigned)(a.B * a.Hk), (unsigned)pblocks), dim3(64 * nw),
                        win_prompt_lds(a.D), st, a);
-    s = launch_status();
-  } else if (p.rt && whole && p.rblocks <= 65535) {
+    return launch_status();
+  }
+  if (p.rt && whole && p.rblocks <= 65535) {
     a.rblocks = p.rblocks;
+    a.rp = 16 * p.rt;
     a.nchunks = p.nchunks;
-    a.part = (float *)(w8 + p.part_off);
-    a.pml = (float *)(w8 + p.pml_off);
     const bool paged = a.table != nullptr;
-    hipLaunchKernelGGL(win_split_pick(dt, a.D, p.rt, paged),
+    hipLaunchKernelGGL(win_split_pick(dt, a.D, p.rt, paged, p.nw),
                        dim3((unsigned)(a.B * a.Hk), (unsigned)p.rblocks, (unsigned)p.nchunks),
-                       dim3(64 * kWinSplitWaves), 0, st, a);
+                       dim3(64 * p.nw), 0, st, a);
     s = launch_status();
-    if (s == MTP_OK && p.nchunks > 1) {
-      hipLaunchKernelGGL(win_merge_pick(dt, a.D, p.rt, paged), dim3((unsigned)((rows + 3) / 4)),
+    if (s == MTP_OK && (p.nchunks > 1 || a.weights)) {
+      // four waves to a row while the chip has room for them
+      const int mw = rows <= 8 * (int64_t)device_cus() ? 4 : 1;
+      a.joins = p.nchunks > 1 ? (int)((rows * mw + 3) / 4) : 0;
+      const int64_t sums = a.weights ? (p.ld_sc + 255) / 256 * a.B * a.Hk : 0;
+      if (a.joins + sums > INT32_MAX) return MTP_ERR_SHAPE;
+      hipLaunchKernelGGL(win_join_pick(dt, a.D, paged, mw), dim3((unsigned)(a.joins + sums)),
                          dim3(256), 0, st, a);
       s = launch_status();
     }
-  } else {
-    hipLaunchKernelGGL(a.table ? win_generic<true>(a.D) : win_generic<false>(a.D),
-                       dim3((unsigned)rows), dim3(64), win_row_lds(a.D) * 4, st, a, dt);
-    s = launch_status();
+    return s;
   }
+  a.rblocks = 1;
+  a.rp = a.G * a.T;
+  hipLaunchKernelGGL(a.table ? win_generic<true>(a.D) : win_generic<false>(a.D),
+                     dim3((unsigned)rows), dim3(64), win_row_lds(a.D) * 4, st, a, dt);
+  s = launch_status();
   if (s != MTP_OK || !a.weights) return s;
   hipLaunchKernelGGL(win_weights_kernel, dim3((unsigned)((p.ld_sc + 255) / 256),
                                               (unsigned)(a.B * a.Hk)),

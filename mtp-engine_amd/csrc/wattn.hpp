@@ -156,8 +156,8 @@ __device__ __forceinline__ void win_row(const WinArgs &a, int ct, int b, int h, 
     if (d < a.D) store_from_f32(a.out, ct, oo + d, o[e] * inv);
   }
   if (keep && lane == 0) {
-    a.ml[row * 2] = m;
-    a.ml[row * 2 + 1] = l;
+    a.pml[row * 2] = m;
+    a.pml[row * 2 + 1] = l;
   }
 }
 

@@ -32,13 +32,14 @@ struct WinArgs {
   const int64_t *lengths;         // [B] keys and queries of each sequence (dense), or null
   float scale;                    // of the scores, in units of log 2
   float *scores;                  // [B * Hk][G * T][ld_sc] masked scores, or null
-  float *ml;                      // [B * Hk][G * T][2]: maximum and sum of a row, with scores
   int64_t ld_sc;
   float *weights;                 // [B, Hk, L], added to
-  // split kernel: row blocks of a (batch, key head), key chunks of a block
-  int rblocks, nchunks;
-  float *part;                    // [b * Hk + hk][row block][chunk][rows][D], nchunks > 1
-  float *pml;                     // the same with (maximum, sum) for D
+  // rows of a (batch, key head) in rblocks blocks of rp, keys of a block in
+  // nchunks chunks
+  int rblocks, rp, nchunks;
+  float *part;                    // [b * Hk + hk][row block][chunk][rp][D], nchunks > 1
+  float *pml;                     // the same with (maximum, sum) for D; with scores too
+  int joins;                      // workgroups that join chunks, before those for the weights
 };
 
 // The keys that the queries of one sequence see: [0, ns) and [lo, hi), the
@@ -53,17 +54,19 @@ struct WinSpan {
   __host__ __device__ int index(int j) const { return j < ns ? j : j - lo + ns; }
 };
 
-// Rows of the split kernel's tiles and its waves; see wattn_split.hpp.
-constexpr int kWinSplitWaves = 4;
-// Keys of a wave's step: whole K = 32 products (16-bit types), and at most 8
-// KB of K.
+// Keys of a wave's step in the split kernel (wattn_split.hpp): whole K = 32
+// products (16-bit types), and at most 8 KB of K.
 constexpr int win_split_keys(int row_bytes) { return row_bytes > 256 ? 16 : 32; }
 
 typedef void (*WinKernel)(WinArgs);
 // The split kernel for rows of type ct and head dim d in tiles of 16 * rt rows
-// (rt 1 or 2) and the merge of its chunks; null for other shapes.
-WinKernel win_split_pick(int ct, int d, int rt, bool paged);
-WinKernel win_merge_pick(int ct, int d, int rt, bool paged);
+// (rt 1 or 2) with nw waves (4 or 8); null for other shapes. Grid (B * Hk, row
+// blocks, chunks).
+WinKernel win_split_pick(int ct, int d, int rt, bool paged, int nw);
+// The join of its chunks with 1 or 4 waves a row, 4 / waves rows a workgroup,
+// and after those a.joins workgroups one for every 256 keys of a (batch, key
+// head) that adds to the weights.
+WinKernel win_join_pick(int ct, int d, bool paged, int waves);
 
 // The prompt kernel (wattn_prompt.hpp) for 16-bit rows of head dim d in blocks
 // of 32 * nw rows (nw 4 or 8), and the keys of its tiles; null for other

@@ -8,26 +8,25 @@
 // parts, one per workgroup, so that few rows still fill the chip; chunks join
 // in win_merge_kernel, in order. Within a workgroup four waves take steps of
 // SK keys in turn and join at the end; a step has no barrier:
-//   * K rows go from memory to the registers that the matrix product wants
-//     them in: lane l holds bytes 64 c + 16 (l / 16) .. + 15 of key l % 16,
-//     for every 64-byte piece c of the row, one load each.
-//   * S^T[key][row] = K Q^T, 16 x 16 tiles with Q^T in registers: lane l has
-//     keys 4 (l / 16) + i of row l % 16, so a row's maximum takes two lane
-//     swaps and its sum none until the end.
+//   * K and V rows go from memory to registers, whole rows a load, and from
+//     there to the wave's own part of LDS; the next step's rows are asked for
+//     as soon as these have left the registers, their pages one step earlier.
+//   * S^T[key][row] = K Q^T, 16 x 16 tiles: lane l has keys 4 (l / 16) + i of
+//     row l % 16, so a row's maximum takes two lane swaps and its sum none
+//     until the end.
 //   * O^T[d][row] += V^T P^T takes the S^T registers as they are (rounded to
-//     the 16-bit type; fp32 stays). V rows, loaded like K's, pass through the
-//     wave's own part of LDS: 16-bit ones come back by transposing reads, four
-//     keys of one d a lane.
-//   * the next step's K and V are asked for as soon as this step's have left
-//     their registers, before its softmax; the page numbers one step earlier.
+//     the 16-bit type; fp32 stays); 16-bit V comes from LDS by transposing
+//     reads, four keys of one d a lane.
 // The running maximum moves only when a step exceeds it by more than 2^8.
 //
 // Bound: HBM, K and V read once per row block (blocks of one key head run on
-// one XCD and meet in its L2). 16 KB a wave in flight, two or more waves per
-// SIMD.
+// one XCD and meet in its L2). 16 KB a wave in flight, two waves per SIMD.
+// Loads in the order of the K operand (16 rows of 64 bytes each) instead of
+// whole rows, without LDS for K: 106 us against 92 on 131072 keys of 8 heads
+// (537 MB); three waves per SIMD of smaller chunks: 122.
 #pragma once
 
-#include "wattn.hpp"
+#include "wattn_weights.hpp"
 
 namespace mtp {
 
@@ -55,19 +54,28 @@ __device__ __forceinline__ int win_swz(int r) {
   else return ((r >> 2) & 1) | (r & 2) | (((r >> 3) & 1) << 2);
 }
 
-template <int CT, int D, int RT, bool PAGED>
-__global__ void __launch_bounds__(64 * kWinSplitWaves, 2) win_split_kernel(const WinArgs a) {
+// Keys of each chunk of n keys, in whole steps.
+template <int SK>
+__device__ __forceinline__ int win_chunk(int n, int nchunks) {
+  return max(1, ((n + nchunks - 1) / nchunks + SK - 1) / SK) * SK;
+}
+
+template <int CT, int D, int RT, bool PAGED, int NW>
+__global__ void __launch_bounds__(64 * NW, 2) win_split_kernel(const WinArgs a) {
   constexpr int EB = dtype_bytes(CT);
   constexpr int RB = D * EB;           // bytes of a row
   constexpr int NC = RB / 64;          // 64-byte pieces of a row
   constexpr int SK = win_split_keys(RB);
   constexpr int KT = SK / 16;          // key tiles of a step
-  constexpr int NW = kWinSplitWaves;
   constexpr int RP = 16 * RT;
   static_assert(RB % 128 == 0 && (CT == MTP_F32 || KT == 2), "whole products");
-  constexpr int kRegion = SK * RB;     // a wave's V rows
+  constexpr int LPK = RB / 16, KPI = 64 / LPK, NL = SK / KPI;  // loads of K (of V) a step
+  constexpr int kRegion = 2 * SK * RB; // a wave's K and V rows
   constexpr int kMerge = NW * 16 * (D + 4) * 4;
   constexpr int kLds = NW * kRegion > kMerge ? NW * kRegion : kMerge;
+  // two tiles of 256 bytes a row: Q^T from LDS, or the registers run out
+  constexpr bool QL = RT == 2 && RB >= 256;
+  __shared__ u32x4 s_q[QL ? RT * NC * 64 : 1];
   __shared__ __attribute__((aligned(16))) unsigned char lds[kLds];
   __shared__ float s_ml[NW][16][2];
   __shared__ unsigned s_bad[RT];
@@ -81,25 +89,42 @@ __global__ void __launch_bounds__(64 * kWinSplitWaves, 2) win_split_kernel(const
   const int nrows = a.G * a.T, row0 = rb * RP;
   const WinSpan s = win_span(a, b, row0 / a.G, (min(nrows, row0 + RP) - 1) / a.G + 1);
   const int n = s.count();
-  const int per = ((n + a.nchunks - 1) / a.nchunks + SK - 1) / SK * SK;
-  const int c0 = min(n, c * per), c1 = min(n, c0 + per);
-  if (c0 >= c1 && c > 0) return;  // the merge knows (chunk 0 writes rows without keys)
+  const int per = win_chunk<SK>(n, a.nchunks);
+  const int c0 = (int)min((int64_t)n, (int64_t)c * per), c1 = (int)min((int64_t)n, (int64_t)c0 + per);
+  const int64_t unit = (((int64_t)bh * a.rblocks + rb) * a.nchunks + c) * RP;  // its rows' partials
+  if (c0 >= c1 && a.nchunks > 1) {  // a chunk without keys
+    if (th < RP) {
+      a.pml[(unit + th) * 2] = -INFINITY;
+      a.pml[(unit + th) * 2 + 1] = 0.f;
+    }
+    return;
+  }
   const int nst = (c1 - c0 + SK - 1) / SK;
 
   // ---- rows of this lane: r = row0 + 16 rt + l16
   int pos[RT];
-  u32x4 qf[RT][NC];
+  const char *qp[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int r = row0 + 16 * rt + l16, t = r / a.G, h = hk * a.G + (r - t * a.G);
     const bool live = r < nrows && t < s.rows;
     pos[rt] = live ? s.first + t : -1;  // -1 sees nothing
-    const char *const qp = (const char *)a.q + ((int64_t)b * a.q_sb + (int64_t)h * a.q_sh +
-                                                (int64_t)t * a.q_st) * EB + 16 * g;
-#pragma unroll
-    for (int k = 0; k < NC; ++k)
-      qf[rt][k] = live ? *(const u32x4 *)(qp + 64 * k) : u32x4{0u, 0u, 0u, 0u};
+    qp[rt] = live ? (const char *)a.q + ((int64_t)b * a.q_sb + (int64_t)h * a.q_sh +
+                                         (int64_t)t * a.q_st) * EB + 16 * g
+                  : nullptr;
   }
+  // Q^T: piece k of tile rt, all of them, or (QL) each wave some, shared in LDS
+  constexpr int NQ = QL ? (RT * NC + NW - 1) / NW : RT * NC;
+  u32x4 qf[NQ];
+  auto load_q = [&]() {
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+      const int p = QL ? wave + NW * i : i;
+      const char *const at = RT == 2 && p >= NC ? qp[RT - 1] : qp[0];
+      qf[i] = u32x4{0u, 0u, 0u, 0u};
+      if (at && p < RT * NC) qf[i] = *(const u32x4 *)(at + 64 * (p % NC));
+    }
+  };
   const int pmin = s.first + row0 / a.G;  // of the block's first row; its last:
   const int pmax = s.first + min(s.rows, (min(nrows, row0 + RP) - 1) / a.G + 1) - 1;
   // call-wide index of a key's score
@@ -111,47 +136,56 @@ __global__ void __launch_bounds__(64 * kWinSplitWaves, 2) win_split_kernel(const
   const int32_t *const tab = PAGED ? a.table + (int64_t)b * a.ld_tab : nullptr;
   const int pmask = (a.page_size & (a.page_size - 1)) == 0 ? a.page_size - 1 : -1;
 
-  u32x4 kr[KT][NC], vr[KT][NC];
-  int pg[KT];            // pages of the step asked for next
-  uint32_t okn = 0u;     // keys present of the step asked for last: bit 16 kt + key
-  auto index_of = [&](int st, int kt) { return c0 + st * SK + 16 * kt + l16; };
+  // Lane i looks up key i % SK of a step; a load instruction takes KPI whole
+  // rows, LPK lanes each.
+  u32x4 kr[NL], vr[NL];
+  int pg = -1;           // page of the step asked for next
+  uint32_t okn = 0u;     // keys present of the step asked for last
+  auto index_of = [&](int st) { return c0 + st * SK + (lane & (SK - 1)); };
   auto load_pages = [&](int st) {
     if constexpr (PAGED) {
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-        const int i = index_of(st, kt);
-        pg[kt] = i < c1 ? tab[s.key(i)] : -1;
-      }
+      const int i = index_of(st);
+      pg = i < c1 ? tab[s.key(i)] : -1;
     }
   };
-  int64_t ko[KT], vo[KT];
-  bool ok[KT];
-  auto locate = [&](int st) {
-    uint32_t m = 0u;
+  auto shfl64 = [&](int64_t x, int from) {
+    return (int64_t)((uint64_t)(uint32_t)__shfl((int)(x >> 32), from, 64) << 32 |
+                     (uint32_t)__shfl((int)x, from, 64));
+  };
+  auto fetch = [&](int st) {
+    const int i = index_of(st), j = s.key(i);
+    bool ok = i < c1;
+    int64_t ko, vo;
+    if constexpr (PAGED) {
+      ok = ok && pg >= 0 && pg < a.npages;
+      const int in = pmask >= 0 ? (j & pmask) : j % a.page_size;
+      ko = vo = ((int64_t)pg * a.p_sp + kbase + (int64_t)in * a.k_st) * EB;
+    } else {
+      ko = (kbase + (int64_t)j * a.k_st) * EB;
+      vo = (vbase + (int64_t)j * a.v_st) * EB;
+    }
+    okn = (uint32_t)(__ballot(ok) & (SK == 32 ? 0xffffffffull : 0xffffull));
+    // a cache is read once; a prompt's keys again by the next row block
+    auto row16 = [](const void *p, int64_t off) {
+      return PAGED ? ld_nt16((const char *)p + off) : ld16((const char *)p + off);
+    };
+    const bool every = okn == (SK == 32 ? 0xffffffffu : 0xffffu);  // the usual step
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt) {
-      const int i = index_of(st, kt), j = s.key(i);
-      ok[kt] = i < c1;
-      if constexpr (PAGED) {
-        ok[kt] = ok[kt] && pg[kt] >= 0 && pg[kt] < a.npages;
-        const int in = pmask >= 0 ? (j & pmask) : j % a.page_size;
-        ko[kt] = vo[kt] = ((int64_t)pg[kt] * a.p_sp + kbase + (int64_t)in * a.k_st) * EB + 16 * g;
+    for (int n = 0; n < NL; ++n) {
+      const int r = n * KPI + lane / LPK;
+      const int64_t c16 = 16 * (lane % LPK);
+      const int64_t kof = shfl64(ko, r) + c16, vof = PAGED ? kof : shfl64(vo, r) + c16;
+      if (every) {
+        kr[n] = row16(a.k, kof);
+        vr[n] = row16(a.v, vof);
       } else {
-        ko[kt] = (kbase + (int64_t)j * a.k_st) * EB + 16 * g;
-        vo[kt] = (vbase + (int64_t)j * a.v_st) * EB + 16 * g;
+        kr[n] = vr[n] = u32x4{0u, 0u, 0u, 0u};
+        if ((okn >> r) & 1u) {
+          kr[n] = row16(a.k, kof);
+          vr[n] = row16(a.v, vof);
+        }
       }
-      m |= (uint32_t)(__ballot(ok[kt]) & 0xffffull) << (16 * kt);
     }
-    okn = m;
-  };
-  auto fetch = [&](u32x4 (&r)[KT][NC], const void *base, const int64_t (&off)[KT]) {
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-      for (int k = 0; k < NC; ++k) {
-        r[kt][k] = u32x4{0u, 0u, 0u, 0u};
-        if (ok[kt]) r[kt][k] = *(const u32x4 *)((const char *)base + off[kt] + 64 * k);
-      }
   };
 
   // ---- state: of row l16 of each tile
@@ -164,49 +198,59 @@ __global__ void __launch_bounds__(64 * kWinSplitWaves, 2) win_split_kernel(const
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) o[rt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  unsigned char *const vl = lds + wave * kRegion;
+  unsigned char *const kl = lds + wave * kRegion, *const vl = kl + SK * RB;
 
+  load_pages(wave);
+  load_q();
   if (wave < nst) {
-    load_pages(wave);
-    locate(wave);
-    fetch(kr, a.k, ko);
-    fetch(vr, a.v, vo);
+    fetch(wave);
     load_pages(wave + NW);
+  }
+  if constexpr (QL) {
+#pragma unroll
+    for (int i = 0; i < NQ; ++i)
+      if (wave + NW * i < RT * NC) s_q[(wave + NW * i) * 64 + lane] = qf[i];
+    lds_barrier();  // loads in flight go on
   }
   for (int st = wave; st < nst; st += NW) {
     const uint32_t okm = okn;
+    const int i0 = c0 + st * SK;
+    // rows to the wave's part of LDS
+#pragma unroll
+    for (int n = 0; n < NL; ++n) {
+      const int r = n * KPI + lane / LPK;
+      const int at = r * RB + 16 * ((lane % LPK) ^ win_swz<CT, RB>(r));
+      *(u32x4 *)(kl + at) = kr[n];
+      *(u32x4 *)(vl + at) = vr[n];
+    }
+    if (st + NW < nst) {
+      fetch(st + NW);
+      load_pages(st + 2 * NW);
+    }
+    win_wave_sync();
     f32x4 sc[RT][KT];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
+    for (int kt = 0; kt < KT; ++kt) {
+      const int r = 16 * kt + l16;
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-        f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int rt = 0; rt < RT; ++rt) sc[rt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < NC; ++k) {
+      for (int k = 0; k < NC; ++k) {
+        const u32x4 x = *(const u32x4 *)(kl + r * RB + 16 * ((4 * k + g) ^ win_swz<CT, RB>(r)));
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          u32x4 y;
+          if constexpr (QL) y = s_q[(rt * NC + k) * 64 + lane];
+          else y = qf[rt * NC + k];
           if constexpr (CT == MTP_F32) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              x = mfma16_f32(__uint_as_float(kr[kt][k][e]), __uint_as_float(qf[rt][k][e]), x);
+              sc[rt][kt] = mfma16_f32(__uint_as_float(x[e]), __uint_as_float(y[e]), sc[rt][kt]);
           } else {
-            x = mfma16<CT>(kr[kt][k], qf[rt][k], x);
+            sc[rt][kt] = mfma16<CT>(x, y, sc[rt][kt]);
           }
         }
-        sc[rt][kt] = x;
       }
-    // V to the wave's rows in LDS
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-      for (int k = 0; k < NC; ++k) {
-        const int r = 16 * kt + l16;
-        *(u32x4 *)(vl + r * RB + 16 * ((4 * k + g) ^ win_swz<CT, RB>(r))) = vr[kt][k];
-      }
-    const int i0 = c0 + st * SK;
-    if (st + NW < nst) {
-      locate(st + NW);
-      fetch(kr, a.k, ko);
-      fetch(vr, a.v, vo);
-      load_pages(st + 2 * NW);
     }
     // ---- scores in units of log 2; hidden ones -inf
     const int jlo = s.key(i0), jhi = s.key(min(i0 + SK, c1) - 1);
@@ -280,7 +324,6 @@ __global__ void __launch_bounds__(64 * kWinSplitWaves, 2) win_split_kernel(const
       }
     }
     // ---- O^T += V^T P^T
-    win_wave_sync();
     if constexpr (CT == MTP_F32) {
 #pragma unroll
       for (int dt = 0; dt < D / 16; ++dt)
@@ -313,9 +356,10 @@ __global__ void __launch_bounds__(64 * kWinSplitWaves, 2) win_split_kernel(const
     win_wave_sync();
   }
 
-  // ---- the four waves join, one row tile at a time: thread (row, 16 lanes)
-  // takes D / 16 elements of a row over the waves in order
-  const int mr = th >> 4, md = (th & 15) * 4;
+  // ---- the waves join, one row tile at a time: TR threads to a row, each
+  // takes some of its elements over the waves in order
+  constexpr int TR = 4 * NW;
+  const int mr = th / TR, mt = th % TR, md = mt * 4;
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const float ls = sum_over_lane_groups(l[rt]);
@@ -339,15 +383,15 @@ __global__ void __launch_bounds__(64 * kWinSplitWaves, 2) win_split_kernel(const
       L = fmaf(s_ml[w][mr][1], e[w], L);
     }
     const int r = row0 + 16 * rt + mr, t = r / a.G, h = hk * a.G + (r - t * a.G);
+    const int64_t at = unit + 16 * rt + mr;
+    if (mt == 0 && (a.nchunks > 1 || a.scores)) {
+      a.pml[at * 2] = M;
+      a.pml[at * 2 + 1] = L;
+    }
     if (a.nchunks > 1) {
       if (r < nrows) {
-        const int64_t at = (((int64_t)bh * a.rblocks + rb) * a.nchunks + c) * RP + 16 * rt + mr;
-        if ((th & 15) == 0) {
-          a.pml[at * 2] = M;
-          a.pml[at * 2 + 1] = L;
-        }
 #pragma unroll
-        for (int d = md; d < D; d += 64) {
+        for (int d = md; d < D; d += 4 * TR) {
           f32x4 O = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int w = 0; w < NW; ++w)
@@ -360,13 +404,8 @@ __global__ void __launch_bounds__(64 * kWinSplitWaves, 2) win_split_kernel(const
     const float inv = L == 0.f ? 0.f : 1.f / L;
     bool bad = false;
     if (r < nrows) {
-      if (a.scores && (th & 15) == 0) {
-        const int64_t at = (int64_t)bh * nrows + r;
-        a.ml[at * 2] = M;
-        a.ml[at * 2 + 1] = L;
-      }
 #pragma unroll
-      for (int d = md; d < D; d += 64) {
+      for (int d = md; d < D; d += 4 * TR) {
         f32x4 O = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < NW; ++w)
@@ -394,62 +433,91 @@ __global__ void __launch_bounds__(64 * kWinSplitWaves, 2) win_split_kernel(const
   }
 }
 
-// Joins the chunks of the split kernel in order, a wave per row.
-template <int CT, int D, int RT, bool PAGED>
-__global__ void __launch_bounds__(256) win_merge_kernel(const WinArgs a) {
-  constexpr int SK = win_split_keys(D * dtype_bytes(CT));
-  constexpr int RP = 16 * RT, E = D / 64;
+// Joins the chunks of the split kernel: W waves per row take chunks w, w + W,
+// ... and join in order; workgroups from a.joins on add to the weights.
+template <int CT, int D, bool PAGED, int W>
+__global__ void __launch_bounds__(256) win_join_kernel(const WinArgs a) {
+  constexpr int E = D / 64;
   constexpr int F = 8;  // chunks in flight
-  __shared__ float s_row[4][(win_row_lds(D) + 3) & ~3];
+  __shared__ __attribute__((aligned(16))) float s_row[4][(win_row_lds(D) + 3) & ~3];
+  __shared__ float s_a[256], s_b[256];
+  if ((int)blockIdx.x >= a.joins) {
+    const int id = (int)blockIdx.x - a.joins, kbs = (int)((a.ld_sc + 255) / 256);
+    win_weights(a, id / kbs, id % kbs, s_a, s_b);
+    return;
+  }
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nrows = a.G * a.T;
-  const int64_t id = (int64_t)blockIdx.x * 4 + wave;
-  if (id >= (int64_t)a.B * a.Hk * nrows) return;
-  const int bh = (int)(id / nrows), r = (int)(id - (int64_t)bh * nrows);
+  const int64_t id = ((int64_t)blockIdx.x * 4 + wave) / W;
+  const int w = wave % W;
+  const bool live = id < (int64_t)a.B * a.Hk * nrows;  // of a whole row: W divides 4
+  const int bh = live ? (int)(id / nrows) : 0, r = live ? (int)(id - (int64_t)bh * nrows) : 0;
   const int b = bh / a.Hk, hk = bh - b * a.Hk;
-  const int rb = r / RP, row0 = rb * RP, t = r / a.G, h = hk * a.G + (r - t * a.G);
-  const WinSpan s = win_span(a, b, row0 / a.G, (min(nrows, row0 + RP) - 1) / a.G + 1);
-  const int n = s.count();
-  const int per = ((n + a.nchunks - 1) / a.nchunks + SK - 1) / SK * SK;
-  const int nc = n > 0 ? (n + per - 1) / per : 1;
-  const int64_t base = ((int64_t)bh * a.rblocks + rb) * a.nchunks * RP + (r - row0);
+  const int rb = r / a.rp, t = r / a.G, h = hk * a.G + (r - t * a.G);
+  const int nc = live ? a.nchunks : 0;
+  const int64_t base = ((int64_t)bh * a.rblocks + rb) * a.nchunks * a.rp + (r - rb * a.rp);
   float M = -INFINITY;
-  for (int c = lane; c < nc; c += 64) M = fmaxf(M, a.pml[(base + (int64_t)c * RP) * 2]);
-#pragma unroll
-  for (int w = 32; w > 0; w >>= 1) M = fmaxf(M, __shfl_xor(M, w, 64));
-  const float ref = M == -INFINITY ? 0.f : M;
+  for (int c = lane; c < nc; c += 64) M = fmaxf(M, a.pml[(base + (int64_t)c * a.rp) * 2]);
   float L = 0.f, o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
-  for (int q0 = 0; q0 < nc; q0 += 64) {
+  float ref = 0.f;
+  // chunk w + W (q0 + lane) in lane `lane`; a chunk without keys (-inf) has
+  // written no row
+  for (int q0 = 0; w + W * q0 < nc; q0 += 64) {
     float fm = -INFINITY, fl = 0.f;
-    if (q0 + lane < nc) {
-      const int64_t at = (base + (int64_t)(q0 + lane) * RP) * 2;
+    const int mine = w + W * (q0 + lane);
+    if (mine < nc) {
+      const int64_t at = (base + (int64_t)mine * a.rp) * 2;
       fm = a.pml[at];
       fl = a.pml[at + 1];
     }
-    const float f = __builtin_amdgcn_exp2f(fm - ref);
-    L += sum_over_lanes<64>(fl * f);
-    const int most = min(64, nc - q0);
+    const int most = min(64, (nc - w - W * q0 + W - 1) / W);
+    float f = 0.f;
     for (int c = 0; c < most; c += F) {
       float x[F][E];
 #pragma unroll
       for (int u = 0; u < F; ++u)
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          x[u][e] = c + u < most ? a.part[(base + (int64_t)(q0 + c + u) * RP) * D + lane + 64 * e]
-                                 : 0.f;
+        for (int e = 0; e < E; ++e) {
+          x[u][e] = 0.f;
+          if (c + u < most)
+            x[u][e] =
+                a.part[(base + (int64_t)(w + W * (q0 + c + u)) * a.rp) * D + lane + 64 * e];
+        }
+      if (c == 0) {  // the maximum of the row, while the first chunks are on their way
+        if (q0 == 0) {
+#pragma unroll
+          for (int y = 32; y > 0; y >>= 1) M = fmaxf(M, __shfl_xor(M, y, 64));
+          ref = M == -INFINITY ? 0.f : M;
+        }
+        f = __builtin_amdgcn_exp2f(fm - ref);
+        L += sum_over_lanes<64>(fl * f);
+      }
 #pragma unroll
       for (int u = 0; u < F; ++u) {
         const float fc = __shfl(f, (c + u) & 63, 64);
-        if (c + u < most) {
+        const bool has = c + u < most && fc != 0.f;
 #pragma unroll
-          for (int e = 0; e < E; ++e) o[e] = fmaf(x[u][e], fc, o[e]);
-        }
+        for (int e = 0; e < E; ++e) o[e] = has ? fmaf(x[u][e], fc, o[e]) : o[e];
       }
     }
   }
+  if constexpr (W > 1) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) s_row[wave][lane + 64 * e] = o[e];
+    if (lane == 0) s_a[wave] = L;
+    __syncthreads();
+    if (w != 0) return;
+#pragma unroll
+    for (int x = 1; x < W; ++x) {
+      L += s_a[wave + x];
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] += s_row[wave + x][lane + 64 * e];
+    }
+  }
+  if (!live) return;
   const float inv = L == 0.f ? 0.f : 1.f / L;
   const int64_t oo = (int64_t)b * a.o_sb + (int64_t)h * a.o_sh + (int64_t)t * a.o_st;
   bool bad = false;
@@ -459,12 +527,9 @@ __global__ void __launch_bounds__(256) win_merge_kernel(const WinArgs a) {
     bad = bad || !(fabsf(y) < INFINITY);
     store_from_f32(a.out, CT, oo + lane + 64 * e, y);
   }
-  if (a.scores && lane == 0) {
-    a.ml[id * 2] = M;
-    a.ml[id * 2 + 1] = L;
-  }
   // not finite: again without the hidden keys
-  if (__ballot(bad) != 0) win_row<E, PAGED>(a, CT, b, h, t, s, s_row[wave], false);
+  if (__ballot(bad) != 0)
+    win_row<E, PAGED>(a, CT, b, h, t, win_span(a, b), s_row[wave], false);
 }
 
 }  // namespace mtp
