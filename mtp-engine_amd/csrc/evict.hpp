@@ -10,11 +10,12 @@
 //
 // Selection, one workgroup per (sequence, head): a weight as an unsigned
 // integer of the same order, entries that stay whatever their weight at its
-// top, absent ones at zero; a radix select finds the keep-th largest value,
-// eight bits a pass from a histogram in LDS, and a last pass writes the
-// positions of the larger ones and of the first of its equals by a prefix sum
-// over the workgroup. Then the rows move, 16 bytes a lane where the row
-// allows it: that part is bound by HBM.
+// top, absent ones at zero; a radix select finds the keep-th largest value, 11,
+// 11 and 10 bits a pass from a histogram in LDS (the top 11 are the sign, the
+// exponent and two bits more, so that few lanes meet in one counter), and a
+// prefix sum over the workgroup gives the larger ones and the first of its
+// equals their places. A thread keeps its run of entries in registers. Then the
+// rows move, 16 bytes a lane where the row allows it: that part is bound by HBM.
 #pragma once
 
 #include "mtp_common.hpp"
@@ -29,6 +30,7 @@ struct EvictArgs {
   int B, Hk, L, keep, sinks, recent, npages, page_size;
   void *k_pages, *v_pages;     // [P, B, Hk, page_size, D], by bytes: from and to
   int64_t row_bytes;
+  int quads;                   // weights and tables in whole 16 bytes a row
   int32_t *kept;               // [B, Hk, keep], -1 past the new length
   float *out_weights;          // [B, Hk, keep], 0 past it
   int64_t *out_lengths;        // [B]
@@ -36,128 +38,168 @@ struct EvictArgs {
 
 constexpr uint32_t kEvictFixed = 0xffffffffu;  // above every weight, NaN among them
 
-// Entry j's rank as an unsigned integer; 0: no entry.
-__device__ __forceinline__ uint32_t evict_key(const EvictArgs &a, const float *w,
-                                              const int32_t *tab, int n, int j) {
-  if (j >= n) return 0u;
-  const int page = tab[j];
-  if (page < 0 || page >= a.npages) return 0u;
-  if (j < a.sinks || j >= n - a.recent) return kEvictFixed;
-  const float x = w[j];
-  if (x != x) return kEvictFixed - 1;
-  const uint32_t u = x == 0.f ? 0u : __float_as_uint(x);  // -0 ranks with 0
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+// Rank of entry j of weight x on a page, as an unsigned integer; 0: no entry.
+__device__ __forceinline__ uint32_t evict_key(const EvictArgs &a, int n, int j, float x, int page) {
+  const uint32_t bits = x == 0.f ? 0u : __float_as_uint(x);  // -0 ranks with 0
+  uint32_t u = (bits & 0x80000000u) ? ~bits : (bits | 0x80000000u);
+  u = x != x ? kEvictFixed - 1 : u;
+  u = (j < a.sinks) | (j >= n - a.recent) ? kEvictFixed : u;
+  return (j < n) & (page >= 0) & (page < a.npages) ? u : 0u;
 }
 
 constexpr int kEvictThreads = 1024;
 
+// Inclusive sum over the workgroup, and its total; s_sum: one word a wave.
+__device__ __forceinline__ uint32_t evict_scan(uint32_t x, uint32_t *s_sum, uint32_t &total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t y = __shfl_up(x, o, 64);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();  // earlier uses of s_sum
+  if (lane == 63) s_sum[wave] = x;
+  __syncthreads();
+  uint32_t before = 0u;
+  total = 0u;
+#pragma unroll
+  for (int w = 0; w < kEvictThreads / 64; ++w) {
+    const uint32_t y = s_sum[w];
+    before += w < wave ? y : 0u;
+    total += y;
+  }
+  return x + before;
+}
+
+// E: entries of a thread in registers, thread th the entries th * E .. + E - 1
+// (E * kEvictThreads >= L); 0: any number, read again for every pass.
+template <int E>
 __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const EvictArgs a) {
-  __shared__ uint32_t s_hist[256];
-  __shared__ uint32_t s_wave[kEvictThreads / 64][2];
+  constexpr int BINS = 2048;
+  constexpr int COPIES = 4;  // of a histogram, lane l in copy l % 4: fewer lanes meet
+  __shared__ uint32_t s_hist[COPIES][BINS + 16];
+  __shared__ uint32_t s_sum[kEvictThreads / 64];
   __shared__ uint32_t s_pick[2];
-  const int th = threadIdx.x, lane = th & 63, wave = th >> 6;
+  const int th = threadIdx.x;
   const int bh = blockIdx.x, b = bh / a.Hk, h = bh - b * a.Hk;
   const float *const w = a.weights + (int64_t)bh * a.L;
   const int32_t *const tab = a.table + (int64_t)b * a.L;
   const int n = (int)min(max(a.lengths[b], (int64_t)0), (int64_t)a.L);
+  const int each = E ? E : (n + kEvictThreads - 1) / kEvictThreads;
+  const int j0 = min((int64_t)th * each, (int64_t)n);  // the thread's entries: j0 .. j1 - 1
+  const int j1 = min((int64_t)j0 + each, (int64_t)n);
 
-  // the keep-th largest rank: after the pass at bit s, `pre` holds its bits
-  // from s up and `need` how many entries are wanted from those that share
-  // them
-  uint32_t pre = 0u, need = (uint32_t)a.keep;
-  for (int sh = 24; sh >= 0; sh -= 8) {
-    for (int i = th; i < 256; i += kEvictThreads) s_hist[i] = 0u;
-    __syncthreads();
-    const uint32_t mask = sh == 24 ? 0u : ~0u << (sh + 8);
-    for (int j = th; j < n; j += kEvictThreads) {
-      const uint32_t u = evict_key(a, w, tab, n, j);
-      if ((u & mask) == (pre & mask)) atomicAdd(&s_hist[(u >> sh) & 255u], 1u);
-    }
-    __syncthreads();
-    if (th < 64) {
-      // lane i holds bins 255 - 4 i .. 252 - 4 i: a prefix sum from the top
-      uint32_t c[4], sum = 0u;
+  uint32_t key[E ? E : 1];
+  float val[E ? E : 1];
+  if constexpr (E > 0) {
+    // every load before the first use (n - 1 in place of entries past the end)
+    int pg[E];
+    if (a.quads && th * E + E <= n) {  // rows of whole 16 bytes
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        c[i] = s_hist[255 - 4 * lane - i];
-        sum += c[i];
-      }
-      uint32_t incl = sum;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t y = __shfl_up(incl, o, 64);
-        if (lane >= o) incl += y;
-      }
-      uint32_t above = incl - sum;
-      const uint32_t total = __shfl(incl, 63, 64);
-      if (total < need) {  // fewer entries than wanted: all of them (rank 0 is below)
-        if (lane == 0) {
-          s_pick[0] = 0u;
-          s_pick[1] = 0u;
-        }
-      } else if (above < need && incl >= need) {
+      for (int e = 0; e < E; e += 4) {
+        const f32x4 x4 = *(const f32x4 *)(w + th * E + e);
+        const u32x4 p4 = *(const u32x4 *)(tab + th * E + e);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if (above < need && above + c[i] >= need) {
-            s_pick[0] = (uint32_t)(255 - 4 * lane - i);
-            s_pick[1] = need - above;
-          }
-          above += c[i];
+          val[e + i] = x4[i];
+          pg[e + i] = (int)p4[i];
         }
       }
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int j = min(th * E + e, max(n - 1, 0));
+        val[e] = n > 0 ? w[j] : 0.f;
+        pg[e] = n > 0 ? tab[j] : -1;
+      }
     }
+#pragma unroll
+    for (int e = 0; e < E; ++e) key[e] = evict_key(a, n, th * E + e, val[e], pg[e]);
+  }
+  auto each_key = [&](auto f) {  // f(entry, rank, weight) over the thread's entries
+    if constexpr (E > 0) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) f(th * E + e, key[e], val[e]);
+    } else {
+      for (int j = j0; j < j1; ++j) f(j, evict_key(a, n, j, w[j], tab[j]), w[j]);
+    }
+  };
+
+  // thr, need: the entries to keep are those above thr and the first `need` of
+  // its equals. After the pass at bit sh, thr has the bits of the keep-th
+  // largest rank from sh up.
+  uint32_t thr = 0u, need = (uint32_t)a.keep;
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const int sh = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const uint32_t bins = pass == 2 ? 1024u : 2048u;
+    const uint32_t mask = pass == 0 ? 0u : ~0u << (pass == 1 ? 21 : 10);
+#pragma unroll
+    for (int c = 0; c < COPIES; ++c) s_hist[c][th] = s_hist[c][th + 1024] = 0u;
     __syncthreads();
-    if (s_pick[1] == 0u) {
-      pre = 0u;
+    each_key([&](int, uint32_t u, float) {
+      if (u != 0u && (u & mask) == thr) {
+        const uint32_t bin = (u >> sh) & (bins - 1u);
+        // lanes of one bin add once (equal weights, above all zeros)
+        const uint32_t first = (uint32_t)__builtin_amdgcn_readfirstlane((int)bin);
+        const unsigned long long all = __ballot(1);
+        if (__ballot(bin == first) == all) {
+          if ((int)(threadIdx.x & 63) == __builtin_ctzll(all))
+            atomicAdd(&s_hist[0][bin], (uint32_t)__popcll(all));
+        } else {
+          atomicAdd(&s_hist[th % COPIES][bin], 1u);
+        }
+      }
+    });
+    __syncthreads();
+    // from the top: thread th has bins 2047 - 2 th and 2046 - 2 th
+    uint32_t c0 = 0u, c1 = 0u;
+#pragma unroll
+    for (int c = 0; c < COPIES; ++c) {
+      c0 += s_hist[c][BINS - 1 - 2 * th];
+      c1 += s_hist[c][BINS - 2 - 2 * th];
+    }
+    uint32_t total;
+    const uint32_t incl = evict_scan(c0 + c1, s_sum, total);
+    const uint32_t above = incl - c0 - c1;
+    if (total < need) {  // fewer entries than wanted (first pass alone): all of them
+      thr = 0u;
       need = 0u;
       break;
     }
-    pre |= s_pick[0] << sh;
-    need = s_pick[1];
+    if (above < need && incl >= need) {
+      const bool hi = above + c0 >= need;
+      s_pick[0] = (uint32_t)(BINS - 1 - 2 * th - (hi ? 0 : 1));
+      s_pick[1] = need - above - (hi ? 0u : c0);
+    }
     __syncthreads();
+    thr |= s_pick[0] << sh;
+    need = s_pick[1];
   }
-  // rank 0 is no entry: then every entry is above it and none of its equals taken
-  if (pre == 0u) need = 0u;
 
-  // entries above `pre` and the first `need` that equal it, in order
-  uint32_t taken = 0u, equal = 0u;
+  uint32_t over = 0u, same = 0u;
+  each_key([&](int, uint32_t u, float) {
+    over += u > thr;
+    same += (u == thr) & (u != 0u);
+  });
+  uint32_t taken, equals;
+  const uint32_t eb = evict_scan(same, s_sum, equals) - same;  // equals before the thread's
+  const uint32_t mine = over + min(eb + same, need) - min(eb, need);
+  uint32_t at = evict_scan(mine, s_sum, taken) - mine;
+  uint32_t es = eb;
   int32_t *const kept = a.kept + (int64_t)bh * a.keep;
   float *const ow = a.out_weights + (int64_t)bh * a.keep;
-  for (int j0 = 0; j0 < n; j0 += kEvictThreads) {
-    const int j = j0 + th;
-    const uint32_t u = evict_key(a, w, tab, n, j);
-    const bool over = u > pre, same = u == pre && pre != 0u;
-    const unsigned long long mo = __ballot(over), ms = __ballot(same);
-    if (lane == 0) {
-      s_wave[wave][0] = (uint32_t)__popcll(mo);
-      s_wave[wave][1] = (uint32_t)__popcll(ms);
-    }
-    __syncthreads();
-    uint32_t eb = equal, before = taken, et = equal, tt = taken;
-    for (int v = 0; v < kEvictThreads / 64; ++v) {
-      const uint32_t o = s_wave[v][0], s = s_wave[v][1];
-      const uint32_t got = o + min(et + s, need) - min(et, need);
-      if (v < wave) {
-        before += got;
-        eb += s;
-      }
-      tt += got;
-      et += s;
-    }
-    const unsigned long long below = lane == 0 ? 0ull : ~0ull >> (64 - lane);
-    const uint32_t es = eb + (uint32_t)__popcll(ms & below);
-    const bool take = over || (same && es < need);
-    if (take) {
-      const uint32_t at = before + (uint32_t)__popcll(mo & below) + min(es, need) - min(eb, need);
+  each_key([&](int j, uint32_t u, float x) {
+    const bool eq = (u == thr) & (u != 0u);
+    if (u > thr || (eq && es < need)) {
       if (at < (uint32_t)a.keep) {
         kept[at] = j;
-        ow[at] = w[j];
+        ow[at] = x;
       }
+      ++at;
     }
-    taken = tt;
-    equal = et;
-    __syncthreads();
-  }
+    es += eq;
+  });
   for (int j = (int)taken + th; j < a.keep; j += kEvictThreads) {
     kept[j] = -1;
     ow[j] = 0.f;

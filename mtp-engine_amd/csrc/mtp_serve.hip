@@ -222,12 +222,12 @@ int win_launch(WinArgs &a, int dt, void *workspace, size_t workspace_bytes, hipS
   const int64_t reach = ((int64_t)1 << 31) / 2 - a.D;
   const bool near = a.k_st >= 0 && a.v_st >= 0 && (a.L - 1) * a.k_st < reach &&
                     (a.L - 1) * a.v_st < reach;
-  const int nw = 8;
-  const WinKernel prompt = a.table || !near ? nullptr : win_prompt_pick(dt, a.D, nw);
-  const int64_t pblocks = ((int64_t)a.G * a.T + 32 * nw - 1) / (32 * nw);
-  if (prompt && whole && (int64_t)a.G * a.T > 128 && pblocks <= 65535) {
+  const WinKernel prompt = a.table || !near ? nullptr : win_prompt_pick(dt, a.D);
+  const int64_t pblocks = ((int64_t)a.G * a.T + kWinPromptRows - 1) / kWinPromptRows;
+  if (prompt && whole && (int64_t)a.G * a.T > kWinPromptRows && pblocks <= 65535) {
     a.rblocks = (int)pblocks;
-    hipLaunchKernelGGL(prompt, dim3((unsigned)(a.B * a.Hk), (unsigned)pblocks), dim3(64 * nw),
+    hipLaunchKernelGGL(prompt, dim3((unsigned)(a.B * a.Hk), (unsigned)pblocks),
+                       dim3(kWinPromptRows * 2),
                        win_prompt_lds(a.D), st, a);
     return launch_status();
   }
@@ -422,7 +422,15 @@ int mtp_kv_evict(const float *weights, const int64_t *lengths, int64_t B, int64_
   const int unit = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : bits % 2 == 0 ? 2 : 1;
   const int64_t blocks = (B * Hk * keep * (row_bytes / unit) + 255) / 256;
   if (blocks > INT32_MAX) return MTP_ERR_SHAPE;
-  hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)(B * Hk)), dim3(kEvictThreads), 0, st, a);
+  a.quads = L % 4 == 0 && aligned16(weights) && aligned16(page_table);
+  // entries of a thread kept in registers, where they fit
+  const int64_t each = (L + kEvictThreads - 1) / kEvictThreads;
+  void (*const sel)(EvictArgs) = each <= 4    ? evict_select_kernel<4>
+                                 : each <= 8  ? evict_select_kernel<8>
+                                 : each <= 16 ? evict_select_kernel<16>
+                                 : each <= 32 ? evict_select_kernel<32>
+                                              : evict_select_kernel<0>;
+  hipLaunchKernelGGL(sel, dim3((unsigned)(B * Hk)), dim3(kEvictThreads), 0, st, a);
   int s = launch_status();
   if (s != MTP_OK || num_pages == 0) return s;
   void (*const mv)(EvictArgs) = unit == 16  ? evict_move_kernel<u32x4>

@@ -68,11 +68,11 @@ WinKernel win_split_pick(int ct, int d, int rt, bool paged, int nw);
 // head) that adds to the weights.
 WinKernel win_join_pick(int ct, int d, bool paged, int waves);
 
-// The prompt kernel (wattn_prompt.hpp) for 16-bit rows of head dim d in blocks
-// of 32 * nw rows (nw 4 or 8), and the keys of its tiles; null for other
-// shapes. Grid (B * Hk, row blocks).
-constexpr int kWinTileKeys = 64;
-WinKernel win_prompt_pick(int ct, int d, int nw);
+// The prompt kernel (wattn_prompt.hpp) for 16-bit rows of head dim d: blocks of
+// kWinPromptRows rows, two threads each, tiles of kWinTileKeys keys; null for
+// other shapes. Grid (B * Hk, row blocks).
+constexpr int kWinPromptRows = 128, kWinTileKeys = 64;
+WinKernel win_prompt_pick(int ct, int d);
 constexpr int win_prompt_lds(int d) { return 2 * 2 * kWinTileKeys * 2 * d; }
 
 }  // namespace mtp

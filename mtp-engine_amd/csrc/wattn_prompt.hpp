@@ -17,6 +17,11 @@
 // The running maximum moves only when a tile exceeds it by more than 2^8. A
 // wave passes over a tile that none of its rows sees. Only tiles at the edge
 // of a wave's window compare positions.
+//
+// Blocks of four waves, two of them on a CU, so that one multiplies while the
+// other is in its softmax: 128 rows against one block of 256 on a CU: 37.5 us
+// against 43.5 (B 4, T 1025, L 2049, H 16, D 64), 85 against 90 (T 4096,
+// window 1024, H 32 / 8, D 128), 420 against 418 (T 8192, window 4096).
 #pragma once
 
 #include "wattn_split.hpp"
@@ -49,7 +54,8 @@ __device__ __forceinline__ void win_dma16(__amdgpu_buffer_rsrc_t r, unsigned cha
 }
 
 template <int CT, int D, int NW>
-__global__ void __launch_bounds__(64 * NW, 2) win_prompt_kernel(const WinArgs a) {
+__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
+win_prompt_kernel(const WinArgs a) {
   constexpr int RB = 2 * D;              // bytes of a row
   constexpr int SK = kWinTileKeys;       // keys of a tile
   constexpr int KBY = SK * RB;           // K bytes of a tile
@@ -79,7 +85,6 @@ __global__ void __launch_bounds__(64 * NW, 2) win_prompt_kernel(const WinArgs a)
   const bool idle = w0 >= nrows || w0 / a.G >= s.rows;
   const int pmin = s.first + w0 / a.G;
   const int pmax = s.first + min(s.rows, (min(nrows, w0 + 32) - 1) / a.G + 1) - 1;
-  const bool full = w0 + 32 <= nrows && (w0 + 31) / a.G < s.rows;
   u32x4 qf[D / 16];
   {
     const uint16_t *const qp = (const uint16_t *)a.q + (int64_t)b * a.q_sb + (int64_t)h * a.q_sh +
@@ -135,15 +140,28 @@ __global__ void __launch_bounds__(64 * NW, 2) win_prompt_kernel(const WinArgs a)
       for (int k = 0; k < D / 16; ++k)
         sc[u] = win_mfma32<CT>(*(const u32x4 *)(krow + 16 * ((2 * k + hi) ^ sw)), qf[k], sc[u]);
     }
-    // hidden scores -inf
-    if (!(full && jhi <= pmin && jlo > pmax - a.window && i0 + SK <= n)) {
+    // hidden scores -inf; a row that is no query's keeps what it has and is
+    // dropped at the end
+    if (!(jhi <= pmin && jlo > pmax - a.window && i0 + SK <= n)) {
+      if (jlo >= a.sinks && jhi - jlo < SK) {
+        // the window alone: distances below the row's position
+        const int d = pos - jlo - 4 * hi, e = min(pos, s.key(n - 1)) - jlo - 4 * hi;
 #pragma unroll
-      for (int u = 0; u < SK / 32; ++u)
+        for (int u = 0; u < SK / 32; ++u)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const int i = i0 + 32 * u + 8 * (v >> 2) + 4 * hi + (v & 3);
-          sc[u][v] = (i < n) & win_sees(a, pos, s.key(i)) ? sc[u][v] : -INFINITY;
-        }
+          for (int v = 0; v < 16; ++v) {
+            const int c = 32 * u + 8 * (v >> 2) + (v & 3);
+            sc[u][v] = (c <= e) & (c > d - a.window) ? sc[u][v] : -INFINITY;
+          }
+      } else {
+#pragma unroll
+        for (int u = 0; u < SK / 32; ++u)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const int i = i0 + 32 * u + 8 * (v >> 2) + 4 * hi + (v & 3);
+            sc[u][v] = (i < n) & win_sees(a, pos, s.key(i)) ? sc[u][v] : -INFINITY;
+          }
+      }
     }
     float mx = sc[0][0];
 #pragma unroll
@@ -221,9 +239,12 @@ __global__ void __launch_bounds__(64 * NW, 2) win_prompt_kernel(const WinArgs a)
     o[dt] *= inv;
 #pragma unroll
     for (int r4 = 0; r4 < 4; ++r4) {
-      const f32x4 x = {o[dt][4 * r4], o[dt][4 * r4 + 1], o[dt][4 * r4 + 2], o[dt][4 * r4 + 3]};
+      f32x4 x = {o[dt][4 * r4], o[dt][4 * r4 + 1], o[dt][4 * r4 + 2], o[dt][4 * r4 + 3]};
 #pragma unroll
-      for (int v = 0; v < 4; ++v) bad = bad || !(fabsf(x[v]) < INFINITY);
+      for (int v = 0; v < 4; ++v) {
+        x[v] = live ? x[v] : 0.f;
+        bad = bad || !(fabsf(x[v]) < INFINITY);
+      }
       if (r < nrows) win_store4<CT>(a, b, h, t, 32 * dt + 8 * r4 + 4 * hi, x);
     }
   }

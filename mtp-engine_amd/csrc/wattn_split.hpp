@@ -254,8 +254,11 @@ __global__ void __launch_bounds__(64 * NW, 2) win_split_kernel(const WinArgs a) 
     }
     // ---- scores in units of log 2; hidden ones -inf
     const int jlo = s.key(i0), jhi = s.key(min(i0 + SK, c1) - 1);
-    const bool all = okm == (KT == 2 ? 0xffffffffu : 0xffffu) && jhi <= pmin &&
-                     jlo > pmax - a.window && row0 + RP <= nrows && s.rows == a.T;
+    // a step that every row sees whole; a row that is no query's keeps what it
+    // has and is dropped at the end
+    const bool all =
+        okm == (KT == 2 ? 0xffffffffu : 0xffffu) && jhi <= pmin && jlo > pmax - a.window;
+    const bool line = jlo >= a.sinks;  // keys jlo, jlo + 1, ...
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
@@ -264,8 +267,8 @@ __global__ void __launch_bounds__(64 * NW, 2) win_split_kernel(const WinArgs a) 
         if (!all) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int j = s.key(i0 + 16 * kt + 4 * g + i);
-            const bool see = (((okm >> (16 * kt + 4 * g + i)) & 1u) != 0) & win_sees(a, pos[rt], j);
+            const int c = 16 * kt + 4 * g + i, j = line ? jlo + c : s.key(i0 + c);
+            const bool see = (((okm >> c) & 1u) != 0) & win_sees(a, pos[rt], j);
             sc[rt][kt][i] = see ? sc[rt][kt][i] : -INFINITY;
           }
         }
@@ -280,9 +283,8 @@ __global__ void __launch_bounds__(64 * NW, 2) win_split_kernel(const WinArgs a) 
         for (int kt = 0; kt < KT; ++kt) {
           const int i = i0 + 16 * kt + 4 * g;
           if (r >= nrows || i >= c1) continue;
-          const int w = whole.index(s.key(i));
-          if (i + 3 < c1 && whole.index(s.key(i + 3)) == w + 3) {
-            *(f32x4u *)(sp + w) = sc[rt][kt];
+          if (line && i0 + SK <= c1) {
+            *(f32x4u *)(sp + whole.index(jlo) + (i - i0)) = sc[rt][kt];
           } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -384,6 +386,8 @@ __global__ void __launch_bounds__(64 * NW, 2) win_split_kernel(const WinArgs a) 
     }
     const int r = row0 + 16 * rt + mr, t = r / a.G, h = hk * a.G + (r - t * a.G);
     const int64_t at = unit + 16 * rt + mr;
+    const bool query = r < nrows && t < s.rows;
+    if (!query) M = -INFINITY, L = 0.f;
     if (mt == 0 && (a.nchunks > 1 || a.scores)) {
       a.pml[at * 2] = M;
       a.pml[at * 2 + 1] = L;
@@ -410,9 +414,11 @@ __global__ void __launch_bounds__(64 * NW, 2) win_split_kernel(const WinArgs a) 
 #pragma unroll
         for (int w = 0; w < NW; ++w)
           O += *(const f32x4 *)((float *)lds + (w * 16 + mr) * (D + 4) + d) * e[w];
-        O *= inv;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) bad = bad || !(fabsf(O[i]) < INFINITY);
+        for (int i = 0; i < 4; ++i) {
+          O[i] = query ? O[i] * inv : 0.f;
+          bad = bad || !(fabsf(O[i]) < INFINITY);
+        }
         win_store4<CT>(a, b, h, t, d, O);
       }
     }
