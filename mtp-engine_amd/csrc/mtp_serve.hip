@@ -235,12 +235,21 @@ int win_launch(WinArgs &a, int dt, void *workspace, size_t workspace_bytes, hipS
     a.rblocks = p.rblocks;
     a.rp = 16 * p.rt;
     a.nchunks = p.nchunks;
+    // up to 48 KB of a block's partials the last workgroup joins (against a
+    // second launch: 8 KB 11.5 us and 14.3, 32 KB 32.3 and 32.9, 64 KB both
+    // 88.2), more of them take longer on one CU than the launch (128 KB 18.3 us
+    // and 14.0)
+    const int64_t partial = std::min<int64_t>(16 * p.rt, (int64_t)a.G * a.T) * p.nchunks * a.D * 4;
+    const bool joined = p.nchunks > 1 && !a.weights && partial <= 48 << 10 &&
+                        p.nchunks <= kWinTicketChunks &&
+                        (int64_t)a.B * a.Hk * p.rblocks <= kCounterSlots;
+    a.ticket = joined ? (unsigned *)w8 : nullptr;
     const bool paged = a.table != nullptr;
     hipLaunchKernelGGL(win_split_pick(dt, a.D, p.rt, paged, p.nw),
                        dim3((unsigned)(a.B * a.Hk), (unsigned)p.rblocks, (unsigned)p.nchunks),
                        dim3(64 * p.nw), 0, st, a);
     s = launch_status();
-    if (s == MTP_OK && (p.nchunks > 1 || a.weights)) {
+    if (s == MTP_OK && !joined && (p.nchunks > 1 || a.weights)) {
       // four waves to a row while the chip has room for them
       const int mw = rows <= 8 * (int64_t)device_cus() ? 4 : 1;
       a.joins = p.nchunks > 1 ? (int)((rows * mw + 3) / 4) : 0;
@@ -422,6 +431,10 @@ int mtp_kv_evict(const float *weights, const int64_t *lengths, int64_t B, int64_
   const int unit = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : bits % 2 == 0 ? 2 : 1;
   const int64_t blocks = (B * Hk * keep * (row_bytes / unit) + 255) / 256;
   if (blocks > INT32_MAX) return MTP_ERR_SHAPE;
+  // up to 64 KB of a head's K the selecting workgroup moves its rows itself
+  // (against a second launch: 64 KB of 8 heads 14.4 us and 15.9, 128 KB of 8
+  // 16.7 and 16.5, of 64 heads 21.9 and 17.1)
+  a.moves = num_pages > 0 && unit == 16 && keep * row_bytes <= 64 << 10;
   a.quads = L % 4 == 0 && aligned16(weights) && aligned16(page_table);
   // entries of a thread kept in registers, where they fit
   const int64_t each = (L + kEvictThreads - 1) / kEvictThreads;
@@ -432,7 +445,7 @@ int mtp_kv_evict(const float *weights, const int64_t *lengths, int64_t B, int64_
                                               : evict_select_kernel<0>;
   hipLaunchKernelGGL(sel, dim3((unsigned)(B * Hk)), dim3(kEvictThreads), 0, st, a);
   int s = launch_status();
-  if (s != MTP_OK || num_pages == 0) return s;
+  if (s != MTP_OK || num_pages == 0 || a.moves) return s;
   void (*const mv)(EvictArgs) = unit == 16  ? evict_move_kernel<u32x4>
                                 : unit == 4 ? evict_move_kernel<uint32_t>
                                 : unit == 2 ? evict_move_kernel<uint16_t>

@@ -39,6 +39,8 @@ struct WinArgs {
   int rblocks, rp, nchunks;
   float *part;                    // [b * Hk + hk][row block][chunk][rp][D], nchunks > 1
   float *pml;                     // the same with (maximum, sum) for D; with scores too
+  unsigned *ticket;               // null, or arrivals per (b * Hk + hk, row block): the last
+                                  // workgroup joins the chunks
   int joins;                      // workgroups that join chunks, before those for the weights
 };
 
@@ -63,6 +65,7 @@ typedef void (*WinKernel)(WinArgs);
 // (rt 1 or 2) with nw waves (4 or 8); null for other shapes. Grid (B * Hk, row
 // blocks, chunks).
 WinKernel win_split_pick(int ct, int d, int rt, bool paged, int nw);
+constexpr int kWinTicketChunks = 64;  // chunks of a block at most, with tickets
 // The join of its chunks with 1 or 4 waves a row, 4 / waves rows a workgroup,
 // and after those a.joins workgroups one for every 256 keys of a (batch, key
 // head) that adds to the weights.

@@ -79,6 +79,7 @@ __global__ void __launch_bounds__(64 * NW, 2) win_split_kernel(const WinArgs a) 
   __shared__ __attribute__((aligned(16))) unsigned char lds[kLds];
   __shared__ float s_ml[NW][16][2];
   __shared__ unsigned s_bad[RT];
+  __shared__ int s_last;
 
   const int th = threadIdx.x, lane = th & 63;
   const int wave = __builtin_amdgcn_readfirstlane(th >> 6);
@@ -92,7 +93,7 @@ __global__ void __launch_bounds__(64 * NW, 2) win_split_kernel(const WinArgs a) 
   const int per = win_chunk<SK>(n, a.nchunks);
   const int c0 = (int)min((int64_t)n, (int64_t)c * per), c1 = (int)min((int64_t)n, (int64_t)c0 + per);
   const int64_t unit = (((int64_t)bh * a.rblocks + rb) * a.nchunks + c) * RP;  // its rows' partials
-  if (c0 >= c1 && a.nchunks > 1) {  // a chunk without keys
+  if (c0 >= c1 && a.nchunks > 1 && !a.ticket) {  // a chunk without keys
     if (th < RP) {
       a.pml[(unit + th) * 2] = -INFINITY;
       a.pml[(unit + th) * 2 + 1] = 0.f;
@@ -388,7 +389,10 @@ __global__ void __launch_bounds__(64 * NW, 2) win_split_kernel(const WinArgs a) 
     const int64_t at = unit + 16 * rt + mr;
     const bool query = r < nrows && t < s.rows;
     if (!query) M = -INFINITY, L = 0.f;
-    if (mt == 0 && (a.nchunks > 1 || a.scores)) {
+    if (mt == 0 && a.ticket) {
+      pub_f32(a.pml + at * 2, M);
+      pub_f32(a.pml + at * 2 + 1, L);
+    } else if (mt == 0 && (a.nchunks > 1 || a.scores)) {
       a.pml[at * 2] = M;
       a.pml[at * 2 + 1] = L;
     }
@@ -400,7 +404,12 @@ __global__ void __launch_bounds__(64 * NW, 2) win_split_kernel(const WinArgs a) 
 #pragma unroll
           for (int w = 0; w < NW; ++w)
             O += *(const f32x4 *)((float *)lds + (w * 16 + mr) * (D + 4) + d) * e[w];
-          *(f32x4 *)(a.part + at * D + d) = O;
+          if (a.ticket) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) pub_f32(a.part + at * D + d + i, O[i]);
+          } else {
+            *(f32x4 *)(a.part + at * D + d) = O;
+          }
         }
       }
       continue;
@@ -424,7 +433,63 @@ __global__ void __launch_bounds__(64 * NW, 2) win_split_kernel(const WinArgs a) 
     }
     if (bad) atomicOr(&s_bad[rt], 1u << mr);
   }
-  if (a.nchunks > 1) return;
+  if (a.nchunks > 1) {
+    if (!a.ticket) return;
+    // ---- the last workgroup of the block to arrive joins its chunks, in order
+    // (the hand-off of mtp_common.hpp)
+    wait_stores();
+    __syncthreads();
+    unsigned *const tk = a.ticket + (int64_t)bh * a.rblocks + rb;
+    if (th == 0) s_last = ticket_add(tk) == (unsigned)a.nchunks - 1;
+    __syncthreads();
+    if (!s_last) return;
+    if (th == 0) ticket_reset(tk);
+    const int64_t base = unit - (int64_t)c * RP;  // the block's first chunk
+    const int nr = min(RP, nrows - row0), nc = a.nchunks;
+    float *const s_f = (float *)lds;  // [row][chunk] maximum, sum
+    static_assert(RP * kWinTicketChunks * 8 <= kLds, "the chunks' maxima and sums");
+    for (int i = th; i < nr * nc; i += 64 * NW) {
+      const int64_t at = (base + (int64_t)(i % nc) * RP + i / nc) * 2;
+      s_f[2 * i] = get_f32(a.pml + at);
+      s_f[2 * i + 1] = get_f32(a.pml + at + 1);
+    }
+    __syncthreads();
+    constexpr int F = 8;  // chunks in flight
+    for (int i = th; i < nr * D; i += 64 * NW) {
+      const int rr = i / D, d = i % D;
+      const float *const f = s_f + 2 * rr * nc;
+      const float *const pp = a.part + (base + rr) * D + d;
+      float x[F];
+#pragma unroll
+      for (int u = 0; u < F; ++u) x[u] = get_f32(pp + (int64_t)min(u, nc - 1) * RP * D);
+      float M = -INFINITY, L = 0.f, O = 0.f;
+      for (int q = 0; q < nc; ++q) M = fmaxf(M, f[2 * q]);
+      const float ref = M == -INFINITY ? 0.f : M;
+      for (int q0 = 0; q0 < nc; q0 += F) {
+        float y[F];
+#pragma unroll
+        for (int u = 0; u < F; ++u) y[u] = x[u];
+        if (q0 + F < nc) {
+#pragma unroll
+          for (int u = 0; u < F; ++u)
+            x[u] = get_f32(pp + (int64_t)min(q0 + F + u, nc - 1) * RP * D);
+        }
+#pragma unroll
+        for (int u = 0; u < F; ++u) {
+          if (q0 + u < nc) {
+            const float e = __builtin_amdgcn_exp2f(f[2 * (q0 + u)] - ref);
+            L = fmaf(f[2 * (q0 + u) + 1], e, L);
+            O = e == 0.f ? O : fmaf(y[u], e, O);
+          }
+        }
+      }
+      const float out = L == 0.f ? 0.f : O / L;
+      const int r = row0 + rr, t = r / a.G, h = hk * a.G + (r - t * a.G);
+      store_from_f32(a.out, CT,
+                     (int64_t)b * a.o_sb + (int64_t)h * a.o_sh + (int64_t)t * a.o_st + d, out);
+      if (!(fabsf(out) < INFINITY)) atomicOr(&s_bad[rr / 16], 1u << (rr % 16));
+    }
+  }
   __syncthreads();
   // ---- rows that are not finite: again without their hidden keys
 #pragma unroll

@@ -694,13 +694,16 @@ def _elsewhere(t: torch.Tensor) -> bool:
     return t.is_cuda and t.get_device() != _current_device()
 
 
-def _same_device(first_name: str, first: torch.Tensor, **others) -> None:
+def _same_device(names: str, first: torch.Tensor, *others) -> int:
+    """The device index of `first`, where every other tensor must be too; names
+    are those of all of them, in order."""
     d = first.get_device()
     if d < 0:
-        _on_device(first_name, first)
-    for o in others.values():
+        _on_device(names.split()[0], first)
+    for o in others:
         if o is not None and o.get_device() != d:
-            _on_device(first_name, first, **others)
+            _on_device(names.split()[0], first, **dict(zip(names.split()[1:], others)))
+    return d
 
 
 def _i64(t: torch.Tensor) -> torch.Tensor:
@@ -755,9 +758,11 @@ def _rope_args(name: str, q, k, inv_freq, start, positions, q_weight, k_weight):
     fdt = inv_freq.dtype
     if fdt is not torch.float32 and fdt is not torch.float64:
         raise TypeError(f"{name}: inv_freq must be float32 or float64, got {fdt}")
+    fshape = inv_freq.shape
+    assert len(fshape) == 1 and 2 * fshape[0] <= D, \
+        f"{name}: inv_freq holds at most D / 2 frequencies"
+    rot = 2 * fshape[0]
     inv_freq = inv_freq.contiguous()
-    rot = 2 * inv_freq.numel()
-    assert inv_freq.dim() == 1 and rot <= D, f"{name}: inv_freq holds at most D / 2 frequencies"
     pos_sb = 0
     if positions is not None:
         pd = positions.dim()
@@ -798,8 +803,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor, start
     lib = _lib.load()
     (B, H, Hk, T, D, f, f64, rot, positions, pos_sb, wq, wk, start_dev, per_row,
      start_host) = _rope_args(name, q, k, inv_freq, start, positions, q_weight, k_weight)
-    _same_device("q", q, k=k, inv_freq=f, positions=positions, q_weight=wq, k_weight=wk,
-                 start=start_dev)
+    dev = _same_device("q k inv_freq positions q_weight k_weight start", q, k, f, positions, wq, wk,
+                       start_dev)
     q, q0, q1, q2 = _rows(q)
     k, k0, k1, k2 = _rows(k)
     qo, ko = torch.empty_like(q), torch.empty_like(k)
@@ -810,7 +815,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor, start
         ptr(wq) or 0, ptr(wk) or 0, ptr(positions) or 0, ptr(start_dev) or 0, B, T, H, Hk, D,
         q0, q1, q2, k0, k1, k2, 0, 0, 0, o0, o1, o2, p0, p1, p2, rot, pos_sb, start_host, 0, 1, 0,
         eps, code(q.dtype), f64, bool(interleaved), bool(norm), per_row)
-    s = lib.mtp_qk_norm_rope(args, _lib.stream_handle(q.device))
+    s = lib.mtp_qk_norm_rope(args, _lib.raw_stream(dev))
     if s:
         check(s, name)
     return qo, ko
@@ -841,8 +846,8 @@ def qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, inv_fr
         f"{name}: v must be like k, got {v.dtype} {tuple(v.shape)}"
     page_table, P, pH, ps, L = _pages_arg(name, k_pages, v_pages, page_table, B, D, dt)
     assert pH == Hk, f"{name}: pages of {pH} heads for {Hk}"
-    _same_device("q", q, k=k, v=v, inv_freq=f, positions=positions, q_weight=wq, k_weight=wk,
-                 start=start_dev, k_pages=k_pages, v_pages=v_pages, page_table=page_table)
+    dev = _same_device("q k v inv_freq positions q_weight k_weight start k_pages v_pages page_table",
+                       q, k, v, f, positions, wq, wk, start_dev, k_pages, v_pages, page_table)
     q, q0, q1, q2 = _rows(q)
     k, k0, k1, k2 = _rows(k)
     v, v0, v1, v2 = _rows(v)
@@ -854,13 +859,15 @@ def qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, inv_fr
         ptr(positions) or 0, ptr(start_dev) or 0, B, T, H, Hk, D, q0, q1, q2, k0, k1, k2, v0, v1,
         v2, o0, o1, o2, 0, 0, 0, rot, pos_sb, start_host, P, ps, L, eps, code(dt), f64,
         bool(interleaved), bool(norm), per_row)
-    s = lib.mtp_qk_norm_rope_write(args, _lib.stream_handle(q.device))
+    s = lib.mtp_qk_norm_rope_write(args, _lib.raw_stream(dev))
     if s:
         check(s, name)
     return qo
 
 
 def _window_arg(name: str, window, sinks) -> Tuple[int, int]:
+    if window is None and sinks == 0:
+        return -1, 0
     if window is not None and int(window) < 1:
         raise ValueError(f"{name}: window must be at least 1 (or None), got {window}")
     if int(sinks) < 0:
@@ -869,14 +876,13 @@ def _window_arg(name: str, window, sinks) -> Tuple[int, int]:
     return (-1 if window is None else min(int(window), 1 << 40)), min(int(sinks), 1 << 40)
 
 
-def _window_call(name: str, fn, pack, q: torch.Tensor, sizes, paged: int, weights: int) -> None:
+def _window_call(name: str, fn, pack, q: torch.Tensor, idx: int, sizes, paged: int,
+                 weights: int) -> None:
     """Runs fn(pack(workspace, bytes)) with the stream's workspace as it is, and
     only where that is too small (nothing has run then) asks for its size."""
-    idx = q.get_device()
     stream = _lib.raw_stream(idx)
     ws = _lib.current_workspace(idx, stream)
-    s = fn(pack(ws.data_ptr() if ws is not None else 0, ws.numel() if ws is not None else 0),
-           stream)
+    s = fn(pack(0, 0) if ws is None else pack(ws.data_ptr(), ws.numel()), stream)
     if s == _lib.ERR_WORKSPACE:
         n = _lib.load().mtp_window_attention_workspace_bytes(code(q.dtype), *sizes, paged, weights)
         at, stream = _lib.scratch(q, n)
@@ -914,7 +920,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     if lengths is not None:
         lengths = _i64(lengths)
         assert tuple(lengths.shape) == (B,), f"{name}: lengths must be [{B}]"
-    _same_device("q", q, k=k, v=v, lengths=lengths)
+    dev = _same_device("q k v lengths", q, k, v, lengths)
     q, q0, q1, q2 = _rows(q)
     k, k0, k1, k2 = _rows(k)
     v, v0, v1, v2 = _rows(v)
@@ -930,7 +936,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                                      q0, q1, q2, k0, k1, k2, v0, v1, v2, o0, o1, o2, win, sinks, 0,
                                      0, 1, scale, cd, 0)
 
-    _window_call(name, lib.mtp_window_attention, pack, q, (B, H, Hk, T, D, L, win, sinks), 0, 0)
+    _window_call(name, lib.mtp_window_attention, pack, q, dev,
+                 (B, H, Hk, T, D, L, win, sinks), 0, 0)
     return out
 
 
@@ -966,8 +973,8 @@ def paged_window_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
         assert weights.shape == (B, Hk, L) and weights.dtype is torch.float32 and \
             weights.is_contiguous(), f"{name}: weights must be contiguous float32 [{B}, {Hk}, {L}]"
         wp = weights.data_ptr()
-    _same_device("q", q, k_pages=k_pages, v_pages=v_pages, page_table=page_table, start=start_dev,
-                 weights=weights)
+    dev = _same_device("q k_pages v_pages page_table start weights", q, k_pages, v_pages, page_table,
+                       start_dev, weights)
     q, q0, q1, q2 = _rows(q)
     if scale is None:
         scale = 1.0 / math.sqrt(D)
@@ -982,8 +989,8 @@ def paged_window_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
                                      q0, q1, q2, 0, 0, 0, 0, 0, 0, o0, o1, o2, win, sinks,
                                      start_host, P, ps, scale, cd, per_row)
 
-    _window_call(name, lib.mtp_paged_window_attention, pack, q, (B, H, Hk, T, D, L, win, sinks), 1,
-                 int(wp != 0))
+    _window_call(name, lib.mtp_paged_window_attention, pack, q, dev,
+                 (B, H, Hk, T, D, L, win, sinks), 1, int(wp != 0))
     return out
 
 
@@ -1028,16 +1035,15 @@ def kv_evict(weights: torch.Tensor, lengths: torch.Tensor, k_pages: torch.Tensor
         raise ValueError(f"{name}: sinks {sinks} and recent {recent} must fit in keep {keep}")
     lengths = _i64(lengths)
     assert lengths.dim() == 1 and lengths.shape[0] == B, f"{name}: lengths must be [{B}]"
-    _same_device("weights", weights, lengths=lengths, k_pages=k_pages, v_pages=v_pages,
-                 page_table=page_table, out_table=out_table)
+    dev = _same_device("weights lengths k_pages v_pages page_table out_table", weights, lengths,
+                       k_pages, v_pages, page_table, out_table)
     kept = out_table.new_empty((B, Hk, keep))
     w = weights.new_empty((B, Hk, keep))
     n = torch.empty_like(lengths)
     s = lib.mtp_kv_evict(weights.data_ptr(), lengths.data_ptr(), B, Hk, L, keep, sinks, recent,
                          k_pages.data_ptr(), v_pages.data_ptr(), P, ps,
                          D * k_pages.element_size(), page_table.data_ptr(), out_table.data_ptr(),
-                         kept.data_ptr(), w.data_ptr(), n.data_ptr(),
-                         _lib.stream_handle(weights.device))
+                         kept.data_ptr(), w.data_ptr(), n.data_ptr(), _lib.raw_stream(dev))
     if s:
         check(s, name)
     return kept, w, n
