@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstddef>
 
 #include "abi_util.hpp"
@@ -125,9 +126,11 @@ int rope_args(RopeArgs &a, const mtp_rope_args *p) {
 
 // ---- windowed attention
 struct WinPlan {
-  int rt = 0;              // split kernel: row tiles of a block; 0: one wave per row
+  bool prompt = false;     // the prompt kernel, where the strides let it
+  int rt = 0;              // else the split kernel: row tiles of a block; 0: one wave per row
   int nw = 4;              // its waves
   int rblocks = 1, nchunks = 1;
+  bool joined = false;     // its chunks joined by their last workgroup
   int64_t ld_sc = 0;       // scores (with weights)
   size_t sc_off = 0, part_off = 0, pml_off = 0, total = 0;
 };
@@ -142,26 +145,56 @@ int win_window(int64_t window) {
   return window < 0 || window >= kWinNone / 2 ? kWinNone : (int)window;
 }
 
-// Rows of 16 whole bytes at 64 or 128 elements take the split kernel: its
-// workgroups of four waves, two on a CU, and chunks of two steps a wave at
-// least.
+// Whether dense 16-bit rows take the prompt kernel: the estimates of both
+// kernels' times, in us, fitted to 176 sizes (head dim 64 and 128; 1 .. 32
+// (batch, key head) pairs, 33 .. 17500 rows, 33 .. 4000 keys, no window):
+//   prompt  5 + 1.25 a tile of the longest block, or 1.6 a tile over the 512
+//           blocks that run at once (head dim 64: 4, 0.9 and 1.1)
+//   split   8 + 45 a million keys of all the 32-row blocks (head dim 64: 7, 28)
+// e.g. at head dim 128: 32 pairs, T 1000, L 1000: 27.9 and 38.7 us measured; 8
+// pairs, T 1000, L 4000: 85.0 and 50.8; one pair of 33 rows and keys: 5.6, 8.1.
+bool win_takes_prompt(int dt, int64_t units, int64_t G, int64_t T, int64_t D, int64_t L,
+                      int64_t window, int64_t sinks) {
+  if (!win_prompt_pick(dt, (int)std::min<int64_t>(D, 1 << 20))) return false;
+  const double rows = (double)(G * T);
+  const double mean = (double)std::min(win_most(1, L, window, sinks), std::max<int64_t>(1, L - T / 2));
+  const double most = (double)win_most(std::min(T, kWinPromptRows / G + 2), L, window, sinks);
+  const double blocks = std::ceil(rows / kWinPromptRows) * units;
+  const bool small = D == 64;
+  const double prompt = (small ? 4. : 5.) +
+                        std::max((small ? 0.9 : 1.25) * std::ceil(most / kWinTileKeys),
+                                 (small ? 1.1 : 1.6) * blocks * (mean / kWinTileKeys + 1.) / 512.);
+  const double split = (small ? 7. : 8.) +
+                       (small ? 28e-6 : 45e-6) * std::ceil(rows / 32.) * units * (mean + 32.);
+  return prompt < split;
+}
+
+// Rows of 16 whole bytes at 64 or 128 elements take the split kernel, dense
+// 16-bit ones the prompt kernel where it is faster.
 WinPlan win_plan(int dt, int64_t B, int64_t H, int64_t Hk, int64_t T, int64_t D, int64_t L,
-                 int window, int64_t sinks, bool weights) {
+                 int window, int64_t sinks, bool paged, bool weights) {
   WinPlan p;
   if (B <= 0 || H <= 0 || Hk <= 0 || H % Hk != 0 || T <= 0 || L <= 0) return p;
   const int64_t rows = H / Hk * T, units = B * Hk;
   size_t at = kCounterBytes;
   if (win_split_pick(dt, (int)std::min<int64_t>(D, 1 << 20), 1, false, 4)) {
+    p.prompt = !paged && win_takes_prompt(dt, units, H / Hk, T, D, L, window, sinks);
     p.rt = rows > 16 ? 2 : 1;
     const int64_t rp = 16 * p.rt;
     p.rblocks = (int)((rows + rp - 1) / rp);
     const int64_t most = win_most(std::min(T, (rp - 1) / (H / Hk) + 2), L, window, sinks);
-    const int64_t wgs = units * p.rblocks, sk = win_split_keys((int)D * dtype_bytes(dt));
+    const int64_t wgs = units * p.rblocks, sk = win_split_keys(dt);
     // eight waves, a workgroup a CU, where that many workgroups suffice (chunks
     // of a step for every wave); else four, so that two of them share a CU
     p.nw = wgs <= device_cus() ? 8 : 4;
     const int64_t room = 8 / p.nw * (int64_t)device_cus() / wgs;
-    p.nchunks = (int)std::max<int64_t>(1, std::min(room, most / (8 * sk)));
+    // (the prompt kernel needs no chunks; a call that it cannot take has one)
+    if (!p.prompt) p.nchunks = (int)std::max<int64_t>(1, std::min(room, most / (8 * sk)));
+    // up to 128 KB of a block's partials the last workgroup joins, more of them
+    // take longer on one CU than a launch of their own (8 KB: 23.9 us and 25.3;
+    // 32 KB: 15.0 and 15.6; 128 KB: 12.2 and 13.8; 256 KB: 16.7 and 14.8)
+    p.joined = p.nchunks > 1 && !weights && p.nchunks <= kWinTicketChunks &&
+               std::min(rp, rows) * p.nchunks * D * 4 <= 128 << 10 && wgs <= kCounterSlots;
     const int64_t parts = wgs * p.nchunks * rp;
     if (p.nchunks > 1) {
       p.part_off = at;
@@ -201,7 +234,7 @@ constexpr int64_t kWinMaxD = 1024;
 
 int win_launch(WinArgs &a, int dt, void *workspace, size_t workspace_bytes, hipStream_t st) {
   const WinPlan p = win_plan(dt, a.B, a.H, a.Hk, a.T, a.D, a.L, a.window, a.sinks,
-                             a.weights != nullptr);
+                             a.table != nullptr, a.weights != nullptr);
   if (p.total > 0 && (!workspace || workspace_bytes < p.total)) return MTP_ERR_WORKSPACE;
   const int64_t rows = (int64_t)a.B * a.H * a.T;
   if (rows > INT32_MAX) return MTP_ERR_SHAPE;
@@ -222,11 +255,10 @@ int win_launch(WinArgs &a, int dt, void *workspace, size_t workspace_bytes, hipS
   const int64_t reach = ((int64_t)1 << 31) / 2 - a.D;
   const bool near = a.k_st >= 0 && a.v_st >= 0 && (a.L - 1) * a.k_st < reach &&
                     (a.L - 1) * a.v_st < reach;
-  const WinKernel prompt = a.table || !near ? nullptr : win_prompt_pick(dt, a.D);
   const int64_t pblocks = ((int64_t)a.G * a.T + kWinPromptRows - 1) / kWinPromptRows;
-  if (prompt && whole && (int64_t)a.G * a.T > kWinPromptRows && pblocks <= 65535) {
+  if (p.prompt && near && whole && pblocks <= 65535) {
     a.rblocks = (int)pblocks;
-    hipLaunchKernelGGL(prompt, dim3((unsigned)(a.B * a.Hk), (unsigned)pblocks),
+    hipLaunchKernelGGL(win_prompt_pick(dt, a.D), dim3((unsigned)(a.B * a.Hk), (unsigned)pblocks),
                        dim3(kWinPromptRows * 2),
                        win_prompt_lds(a.D), st, a);
     return launch_status();
@@ -235,23 +267,15 @@ int win_launch(WinArgs &a, int dt, void *workspace, size_t workspace_bytes, hipS
     a.rblocks = p.rblocks;
     a.rp = 16 * p.rt;
     a.nchunks = p.nchunks;
-    // up to 48 KB of a block's partials the last workgroup joins (against a
-    // second launch: 8 KB 11.5 us and 14.3, 32 KB 32.3 and 32.9, 64 KB both
-    // 88.2), more of them take longer on one CU than the launch (128 KB 18.3 us
-    // and 14.0)
-    const int64_t partial = std::min<int64_t>(16 * p.rt, (int64_t)a.G * a.T) * p.nchunks * a.D * 4;
-    const bool joined = p.nchunks > 1 && !a.weights && partial <= 48 << 10 &&
-                        p.nchunks <= kWinTicketChunks &&
-                        (int64_t)a.B * a.Hk * p.rblocks <= kCounterSlots;
-    a.ticket = joined ? (unsigned *)w8 : nullptr;
+    a.ticket = p.joined ? (unsigned *)w8 : nullptr;
     const bool paged = a.table != nullptr;
     hipLaunchKernelGGL(win_split_pick(dt, a.D, p.rt, paged, p.nw),
                        dim3((unsigned)(a.B * a.Hk), (unsigned)p.rblocks, (unsigned)p.nchunks),
                        dim3(64 * p.nw), 0, st, a);
     s = launch_status();
-    if (s == MTP_OK && !joined && (p.nchunks > 1 || a.weights)) {
-      // four waves to a row while the chip has room for them
-      const int mw = rows <= 8 * (int64_t)device_cus() ? 4 : 1;
+    if (s == MTP_OK && !p.joined && (p.nchunks > 1 || a.weights)) {
+      // four waves to a row of many chunks while the chip has room for them
+      const int mw = p.nchunks > 8 && rows <= 8 * (int64_t)device_cus() ? 4 : 1;
       a.joins = p.nchunks > 1 ? (int)((rows * mw + 3) / 4) : 0;
       const int64_t sums = a.weights ? (p.ld_sc + 255) / 256 * a.B * a.Hk : 0;
       if (a.joins + sums > INT32_MAX) return MTP_ERR_SHAPE;
@@ -346,11 +370,10 @@ int mtp_qk_norm_rope_write(const mtp_rope_args *p, void *stream) {
 size_t mtp_window_attention_workspace_bytes(int dtype, int64_t B, int64_t H, int64_t Hk, int64_t T,
                                             int64_t D, int64_t L, int64_t window, int64_t sinks,
                                             int paged, int weights) {
-  (void)paged;
   if (!is_float_dt(dtype) || T > kWinMaxKeys || L > kWinMaxKeys || B > INT32_MAX || H > 65535)
     return 0;
   return win_plan(dtype, B, H, Hk, T, D, L, win_window(window), std::max<int64_t>(sinks, 0),
-                  weights != 0)
+                  paged != 0, weights != 0)
       .total;
 }
 

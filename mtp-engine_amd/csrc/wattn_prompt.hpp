@@ -25,7 +25,6 @@
 #pragma once
 
 #include "wattn_split.hpp"
-#include "wstream.hpp"
 
 namespace mtp {
 

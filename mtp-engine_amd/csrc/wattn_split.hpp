@@ -27,6 +27,7 @@
 #pragma once
 
 #include "wattn_weights.hpp"
+#include "wstream.hpp"
 
 namespace mtp {
 
@@ -65,7 +66,7 @@ __global__ void __launch_bounds__(64 * NW, 2) win_split_kernel(const WinArgs a) 
   constexpr int EB = dtype_bytes(CT);
   constexpr int RB = D * EB;           // bytes of a row
   constexpr int NC = RB / 64;          // 64-byte pieces of a row
-  constexpr int SK = win_split_keys(RB);
+  constexpr int SK = win_split_keys(CT);
   constexpr int KT = SK / 16;          // key tiles of a step
   constexpr int RP = 16 * RT;
   static_assert(RB % 128 == 0 && (CT == MTP_F32 || KT == 2), "whole products");
@@ -359,6 +360,11 @@ __global__ void __launch_bounds__(64 * NW, 2) win_split_kernel(const WinArgs a) 
     win_wave_sync();
   }
 
+  // the block's partials, with tickets: 16 bytes a lane at the device's
+  // coherence point (the hand-off of mtp_common.hpp)
+  const __amdgpu_buffer_rsrc_t prs =
+      make_rsrc(a.part + (unit - (int64_t)c * RP) * D,
+                a.ticket ? (uint32_t)a.nchunks * (uint32_t)(RP * D * 4) : 0u);
   // ---- the waves join, one row tile at a time: TR threads to a row, each
   // takes some of its elements over the waves in order
   constexpr int TR = 4 * NW;
@@ -405,8 +411,9 @@ __global__ void __launch_bounds__(64 * NW, 2) win_split_kernel(const WinArgs a) 
           for (int w = 0; w < NW; ++w)
             O += *(const f32x4 *)((float *)lds + (w * 16 + mr) * (D + 4) + d) * e[w];
           if (a.ticket) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) pub_f32(a.part + at * D + d + i, O[i]);
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, O), prs,
+                                                   (uint32_t)((c * RP + 16 * rt + mr) * D + d) * 4u,
+                                                   0, kSc1);
           } else {
             *(f32x4 *)(a.part + at * D + d) = O;
           }
@@ -436,7 +443,6 @@ __global__ void __launch_bounds__(64 * NW, 2) win_split_kernel(const WinArgs a) 
   if (a.nchunks > 1) {
     if (!a.ticket) return;
     // ---- the last workgroup of the block to arrive joins its chunks, in order
-    // (the hand-off of mtp_common.hpp)
     wait_stores();
     __syncthreads();
     unsigned *const tk = a.ticket + (int64_t)bh * a.rblocks + rb;
@@ -448,46 +454,55 @@ __global__ void __launch_bounds__(64 * NW, 2) win_split_kernel(const WinArgs a) 
     const int nr = min(RP, nrows - row0), nc = a.nchunks;
     float *const s_f = (float *)lds;  // [row][chunk] maximum, sum
     static_assert(RP * kWinTicketChunks * 8 <= kLds, "the chunks' maxima and sums");
+    constexpr int F = 8, Q = D / 4;  // chunks in flight; four elements a thread
+    auto fetch4 = [&](f32x4 (&x)[F], int q0, int i) {
+#pragma unroll
+      for (int u = 0; u < F; ++u)
+        x[u] = __builtin_bit_cast(
+            f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                       prs, (uint32_t)((min(q0 + u, nc - 1) * RP + i / Q) * D + i % Q * 4) * 4u, 0,
+                       kSc1));
+    };
+    f32x4 x[F];
+    fetch4(x, 0, min(th, nr * Q - 1));
     for (int i = th; i < nr * nc; i += 64 * NW) {
       const int64_t at = (base + (int64_t)(i % nc) * RP + i / nc) * 2;
       s_f[2 * i] = get_f32(a.pml + at);
       s_f[2 * i + 1] = get_f32(a.pml + at + 1);
     }
     __syncthreads();
-    constexpr int F = 8;  // chunks in flight
-    for (int i = th; i < nr * D; i += 64 * NW) {
-      const int rr = i / D, d = i % D;
+    for (int i = th; i < nr * Q; i += 64 * NW) {
+      if (i != th) fetch4(x, 0, i);
+      const int rr = i / Q, d = i % Q * 4;
       const float *const f = s_f + 2 * rr * nc;
-      const float *const pp = a.part + (base + rr) * D + d;
-      float x[F];
-#pragma unroll
-      for (int u = 0; u < F; ++u) x[u] = get_f32(pp + (int64_t)min(u, nc - 1) * RP * D);
-      float M = -INFINITY, L = 0.f, O = 0.f;
+      float M = -INFINITY, L = 0.f;
+      f32x4 O = f32x4{0.f, 0.f, 0.f, 0.f};
       for (int q = 0; q < nc; ++q) M = fmaxf(M, f[2 * q]);
       const float ref = M == -INFINITY ? 0.f : M;
       for (int q0 = 0; q0 < nc; q0 += F) {
-        float y[F];
+        f32x4 y[F];
 #pragma unroll
         for (int u = 0; u < F; ++u) y[u] = x[u];
-        if (q0 + F < nc) {
-#pragma unroll
-          for (int u = 0; u < F; ++u)
-            x[u] = get_f32(pp + (int64_t)min(q0 + F + u, nc - 1) * RP * D);
-        }
+        if (q0 + F < nc) fetch4(x, q0 + F, i);
 #pragma unroll
         for (int u = 0; u < F; ++u) {
           if (q0 + u < nc) {
             const float e = __builtin_amdgcn_exp2f(f[2 * (q0 + u)] - ref);
             L = fmaf(f[2 * (q0 + u) + 1], e, L);
-            O = e == 0.f ? O : fmaf(y[u], e, O);
+            if (e != 0.f) O += y[u] * e;
           }
         }
       }
-      const float out = L == 0.f ? 0.f : O / L;
       const int r = row0 + rr, t = r / a.G, h = hk * a.G + (r - t * a.G);
-      store_from_f32(a.out, CT,
-                     (int64_t)b * a.o_sb + (int64_t)h * a.o_sh + (int64_t)t * a.o_st + d, out);
-      if (!(fabsf(out) < INFINITY)) atomicOr(&s_bad[rr / 16], 1u << (rr % 16));
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+      bool bad = false;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        O[j] *= inv;
+        bad = bad || !(fabsf(O[j]) < INFINITY);
+      }
+      win_store4<CT>(a, b, h, t, d, O);
+      if (bad) atomicOr(&s_bad[rr / 16], 1u << (rr % 16));
     }
   }
   __syncthreads();
