@@ -256,7 +256,8 @@ int win_launch(WinArgs &a, int dt, void *workspace, size_t workspace_bytes, hipS
   const bool near = a.k_st >= 0 && a.v_st >= 0 && (a.L - 1) * a.k_st < reach &&
                     (a.L - 1) * a.v_st < reach;
   const int64_t pblocks = ((int64_t)a.G * a.T + kWinPromptRows - 1) / kWinPromptRows;
-  if (p.prompt && near && whole && pblocks <= 65535) {
+  // (its maximum is that of the products, so it takes no scale below zero)
+  if (p.prompt && near && whole && a.scale > 0.f && pblocks <= 65535) {
     a.rblocks = (int)pblocks;
     hipLaunchKernelGGL(win_prompt_pick(dt, a.D), dim3((unsigned)(a.B * a.Hk), (unsigned)pblocks),
                        dim3(kWinPromptRows * 2),

@@ -159,7 +159,8 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeArgs a) {
     }
   }
   // y = rs * (x * A + partner * B): A the gain times cos, B the partner's gain
-  // times -+ sin, for queries and for keys
+  // times -+ sin, for queries and for keys; a chunk that is not rotated has
+  // zeros for its partner, as it may hold an infinity itself
   float A[2][VEC], B[2][VEC];
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
@@ -213,11 +214,14 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeArgs a) {
     }
     if constexpr (INTER) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) y[i] = x[i ^ 1];
+      for (int i = 0; i < VEC; ++i) y[i] = rotated ? x[i ^ 1] : 0.f;
     } else {
       u32x4 o;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = __shfl(raw[i], mate, 64);
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t z = __shfl(raw[i], mate, 64);
+        o[i] = rotated ? z : 0u;
+      }
       rope_unpack<DT>(o, y);
     }
 #pragma unroll

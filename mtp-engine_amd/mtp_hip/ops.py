@@ -691,7 +691,8 @@ _current_device = getattr(torch._C, "_cuda_getDevice", lambda: -1)
 def _elsewhere(t: torch.Tensor) -> bool:
     """t is on a HIP device that is not the current one: a launch goes to the
     current device, whatever its stream."""
-    return t.is_cuda and t.get_device() != _current_device()
+    d = t.get_device()
+    return d >= 0 and d != _current_device()
 
 
 def _same_device(names: str, first: torch.Tensor, *others) -> int:
@@ -713,11 +714,22 @@ def _i64(t: torch.Tensor) -> torch.Tensor:
 
 def _rows(t: torch.Tensor):
     """(t with d contiguous, its batch, head and token strides)"""
-    s = t.stride()
-    if s[3] != 1:
+    s0, s1, s2, s3 = t.stride()
+    if s3 != 1:
         t = t.contiguous()
-        s = t.stride()
-    return t, s[0], s[1], s[2]
+        s0, s1, s2, s3 = t.stride()
+    return t, s0, s1, s2
+
+
+def _like(t: torch.Tensor):
+    """(an output of t's shape with d contiguous, its batch, head and token
+    strides): t's order of dimensions in memory, unless t's rows overlap."""
+    o = torch.empty_like(t)
+    s0, s1, s2, s3 = o.stride()
+    if s3 != 1:
+        o = t.new_empty(t.shape)
+        s0, s1, s2, s3 = o.stride()
+    return o, s0, s1, s2
 
 
 def _start_arg(name: str, start, B: int):
@@ -807,9 +819,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor, start
                        start_dev)
     q, q0, q1, q2 = _rows(q)
     k, k0, k1, k2 = _rows(k)
-    qo, ko = torch.empty_like(q), torch.empty_like(k)
-    o0, o1, o2, _ = qo.stride()
-    p0, p1, p2, _ = ko.stride()
+    qo, o0, o1, o2 = _like(q)
+    ko, p0, p1, p2 = _like(k)
     args = _lib.ROPE_ARGS.pack(
         q.data_ptr(), k.data_ptr(), 0, qo.data_ptr(), ko.data_ptr(), 0, 0, 0, f.data_ptr(),
         ptr(wq) or 0, ptr(wk) or 0, ptr(positions) or 0, ptr(start_dev) or 0, B, T, H, Hk, D,
@@ -851,8 +862,7 @@ def qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, inv_fr
     q, q0, q1, q2 = _rows(q)
     k, k0, k1, k2 = _rows(k)
     v, v0, v1, v2 = _rows(v)
-    qo = torch.empty_like(q)
-    o0, o1, o2, _ = qo.stride()
+    qo, o0, o1, o2 = _like(q)
     args = _lib.ROPE_ARGS.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), qo.data_ptr(), 0, k_pages.data_ptr(),
         v_pages.data_ptr(), page_table.data_ptr(), f.data_ptr(), ptr(wq) or 0, ptr(wk) or 0,
@@ -926,8 +936,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     v, v0, v1, v2 = _rows(v)
     if scale is None:
         scale = 1.0 / math.sqrt(D)
-    out = torch.empty_like(q)
-    o0, o1, o2, _ = out.stride()
+    out, o0, o1, o2 = _like(q)
     qp, kp, vp, op, lp, cd = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                               ptr(lengths) or 0, code(dt))
 
@@ -978,8 +987,7 @@ def paged_window_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     q, q0, q1, q2 = _rows(q)
     if scale is None:
         scale = 1.0 / math.sqrt(D)
-    out = torch.empty_like(q)
-    o0, o1, o2, _ = out.stride()
+    out, o0, o1, o2 = _like(q)
     qp, kp, vp, op, tp, sp, cd = (q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
                                   out.data_ptr(), page_table.data_ptr(), ptr(start_dev) or 0,
                                   code(dt))
@@ -1019,6 +1027,8 @@ def kv_evict(weights: torch.Tensor, lengths: torch.Tensor, k_pages: torch.Tensor
     weights = weights.contiguous()
     B, Hk, L = weights.shape
     D = k_pages.shape[-1]
+    if B and out_table.data_ptr() == page_table.data_ptr():
+        raise ValueError(f"{name}: out_table is page_table: rows cannot move onto themselves")
     page_table, P, pH, ps, _L = _pages_arg(name, k_pages, v_pages, page_table, B, D, k_pages.dtype)
     assert pH == Hk and Hk > 0, f"{name}: pages of {pH} heads for weights of {Hk}"
     assert _L == L, f"{name}: page_table has {_L} != {L} positions"
@@ -1027,8 +1037,6 @@ def kv_evict(weights: torch.Tensor, lengths: torch.Tensor, k_pages: torch.Tensor
         f"{name}: out_table must be [{B}, keep]"
     if out_table.dtype is not torch.int32 or not out_table.is_contiguous():
         out_table = _i32(out_table.contiguous())
-    if B and out_table.data_ptr() == page_table.data_ptr():
-        raise ValueError(f"{name}: out_table is page_table: rows cannot move onto themselves")
     keep = oshape[1]
     sinks, recent = int(sinks), int(recent)
     if sinks < 0 or recent < 0 or sinks + recent > keep:

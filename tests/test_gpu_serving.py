@@ -626,3 +626,147 @@ def test_calls_repeat_bit_for_bit_and_on_other_streams():
     torch.cuda.synchronize()
     for out, w in got:
         assert torch.equal(out, first[0]) and torch.equal(w, first[1])
+
+
+# ---------------------------------------------------------------------------
+# calls at the edges of what the entry points take
+@pytest.mark.parametrize("dt,D,rot,inter", [(BF16, 64, 32, False), (F32, 64, 16, True),
+                                            (F16, 128, 0, False), (F32, 20, 6, False)])
+def test_elements_past_the_rotation_pass_as_they_are(dt, D, rot, inter):
+    from mtp_hip import ops
+    g = gen(D)
+    x = randn(g, 2, 3, 5, D, dtype=dt)
+    x[0, 1, 2, rot + 3] = math.inf
+    x[1, 2, 4, D - 1] = -math.inf
+    x[1, 0, 0, rot] = math.nan
+    f = inv_freq(rot).to(DEV)
+    for y in ops.qk_norm_rope(x.to(DEV), x.to(DEV), f, 1000, norm=False, interleaved=inter):
+        y = y.cpu()
+        assert torch.equal(y[..., rot:].nan_to_num(nan=7.0), x[..., rot:].nan_to_num(nan=7.0))
+        assert torch.isfinite(y[..., :rot]).all()
+
+
+@pytest.mark.parametrize("dt,D", [(BF16, 64), (F32, 64), (F16, 24)])
+def test_overlapping_and_broadcast_inputs(dt, D):
+    """Sliding views (token stride 1, like the elements') and one key head for all."""
+    from mtp_hip import ops
+    g = gen(21)
+    B, H, Hk, T = 2, 4, 2, 9
+    q = randn(g, B, H, T + D - 1, dtype=dt).to(DEV).unfold(2, D, 1)
+    k = randn(g, B, 1, T, D, dtype=dt).to(DEV).expand(B, Hk, T, D)
+    assert q.stride()[2:] == (1, 1) and k.stride(1) == 0
+    f = inv_freq(D).to(DEV)
+    pos = torch.arange(T).expand(B, T)
+    qo, ko = ops.qk_norm_rope(q, k, f)
+    for y, x in ((qo, q), (ko, k)):
+        ref, mag = S.norm_rotate(x, None, pos, inv_freq(D))
+        within(y, ref, rope_bound(ref, mag, dt))
+    out = ops.window_attention(q, k, k, 4, 1)
+    see = S.visible([0] * B, [T] * B, T, T, 4, 1)
+    attn_check(out, q, k, k, see, dt)
+    kp, vp, table, _ = make_pages(g, 4, B, Hk, 16, D, 40, dt)
+    out = ops.paged_window_attention(q, kp.to(DEV), vp.to(DEV), table.to(DEV), 16, 30)
+    see = S.visible([30] * B, [T] * B, T, 40, None, 0)
+    attn_check(out, q, S.rows_of(kp, table, 16)[0], S.rows_of(vp, table, 16)[0], see, dt)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3])
+@pytest.mark.parametrize("dt,D", [(BF16, 64), (F16, 128), (F32, 64)])
+def test_window_attention_scales_not_above_zero(dt, D, scale):
+    from mtp_hip import ops
+    g = gen(22)
+    q, k, v = (randn(g, 1, 2, n, D, dtype=dt) for n in (200, 260, 260))
+    out = ops.window_attention(q.to(DEV), k.to(DEV), v.to(DEV), 100, 2, scale=scale)
+    see = S.visible([60], [200], 200, 260, 100, 2)
+    ref, spread, _, _ = S.attention(q, k, v, see, scale=scale)
+    score = S.attention(q, k, v, see, scale=abs(scale))[3]
+    e = (D + 6) * U * score[..., None]
+    h16 = half(dt) if dt is not F32 else 0.0
+    within(out, ref, half(dt) * ref.abs() + (h16 + 2 * e + 272 * U) * spread + 2.0 ** -25)
+
+
+@pytest.mark.parametrize("dt,B,T,L,H,Hk,D,window,sinks", [
+    (BF16, 1, 7, 30, 2, 2, 128, None, 0), (BF16, 3, 20, 20, 4, 4, 64, 5, 1),
+    (F16, 1, 128, 128, 1, 1, 128, None, 0), (BF16, 2, 65, 64 + 65, 2, 1, 64, 64, 0),
+    (F16, 1, 33, 2000, 1, 1, 128, None, 0), (F16, 1, 81, 4091, 4, 2, 64, None, 0),
+    (BF16, 1, 33, 9000, 1, 1, 64, None, 0), (BF16, 1, 40, 3000, 2, 1, 128, 900, 5),
+    (F32, 1, 40, 1500, 1, 1, 64, None, 0), (F32, 1, 9, 700, 2, 1, 128, 300, 1),
+    (BF16, 1, 1, 3000, 2, 1, 64, None, 0)])
+def test_few_rows_of_a_prompt(dt, B, T, L, H, Hk, D, window, sinks):
+    """Short prompts, and a few rows behind many keys: their keys in chunks."""
+    from mtp_hip import ops
+    g = gen(T + L)
+    q, k, v = (randn(g, B, h, n, D, dtype=dt) for h, n in ((H, T), (Hk, L), (Hk, L)))
+    print(f"case rows {dt} {(B, T, L, H, Hk, D, window, sinks)}", flush=True)
+    args = [x.to(DEV) for x in (q, k, v)]
+    see = S.visible([L - T] * B, [T] * B, T, L, window, sinks)
+    out = ops.window_attention(*args, window, sinks)
+    attn_check(out, q, k, v, see, dt)
+    assert torch.equal(out, ops.window_attention(*args, window, sinks))
+    # a NaN value that the first row alone does not see
+    if window is None and T > 1:
+        v[:, :, L - T + 1, 3] = math.nan
+        out = ops.window_attention(args[0], args[1], v.to(DEV)).cpu()
+        assert torch.isnan(out[:, :, 1:, 3]).all() and torch.isfinite(out[:, :, 0]).all()
+
+
+@pytest.mark.parametrize("L,keep", [(4096, 64), (4097, 300), (9000, 65), (20000, 64), (33000, 100)])
+def test_kv_evict_lengths(L, keep):
+    """Entries of a thread in registers (up to 4, 8, 16, 32 of them) or not, and
+    rows moved by the selecting workgroup."""
+    from mtp_hip import ops
+    g = gen(L)
+    B, Hk, D, page = 2, 1, 64, 64
+    P = L // page + keep // page + 4
+    w = torch.randint(0, 200, (B, Hk, L), generator=g).float()
+    kp, vp, table, out_table = make_pages(g, P, B, Hk, page, D, L, BF16, keep)
+    kd, vd = kp.to(DEV), vp.to(DEV)
+    n = [L, L // 2 + 3]
+    got = ops.kv_evict(w.to(DEV), torch.tensor(n).to(DEV), kd, vd, table.to(DEV),
+                       out_table.to(DEV), 4, 20)
+    want = S.evict(w, n, kp, vp, table, out_table, 4, 20)
+    for a, b in zip(got + (kd, vd), want):
+        assert torch.equal(a.cpu(), b)
+
+
+@pytest.mark.parametrize("dt", [BF16, F32])
+def test_pages_past_32_bits(dt):
+    """A pool of more than 2^31 elements, read and written at its far end: the
+    same results as from a small one."""
+    from mtp_hip import ops
+    g = gen(24)
+    B, H, Hk, D, page, L, T, keep = 1, 4, 1, 128, 16, 300, 5, 60
+    small = 64
+    kp, vp, table, out_table = make_pages(g, small, B, Hk, page, D, L, dt, keep)
+    P = 2 ** 31 // (Hk * page * D) + small
+    big = [torch.empty(P, B, Hk, page, D, dtype=dt, device=DEV) for _ in range(2)]
+    for to, x in zip(big, (kp, vp)):
+        to[P - small:] = x.to(DEV)
+    q, k, v = (randn(g, B, h, T, D, dtype=dt).to(DEV) for h in (H, Hk, Hk))
+    f = inv_freq(D).to(DEV)
+    runs = []
+    for (kd, vd), base in (((kp.to(DEV), vp.to(DEV)), 0), (big, P - small)):
+        td, od = (x.to(DEV) + base for x in (table, out_table))
+        w = torch.zeros(B, Hk, L, device=DEV)
+        qr = ops.qk_norm_rope_write(q, k, v, f, kd, vd, td, L - T)
+        out = ops.paged_window_attention(qr, kd, vd, td, page, L - T, weights=w)
+        cut = ops.kv_evict(w, torch.tensor([L]).to(DEV), kd, vd, td, od, 1, 8)
+        runs.append([x.cpu() for x in (qr, out, w, *cut, kd[base:base + small],
+                                       vd[base:base + small])])
+    for a, b in zip(*runs):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dt", [BF16, F32])
+def test_dense_keys_past_32_bits(dt):
+    """Key rows so far apart that their offsets pass 2^31 elements."""
+    from mtp_hip import ops
+    g = gen(25)
+    T, L, D, apart = 200, 270, 64, 1 << 23
+    q, k, v = (randn(g, 1, 1, n, D, dtype=dt) for n in (T, L, L))
+    room = torch.empty((L - 1) * apart + 2 * D, dtype=dt, device=DEV)
+    rows = room.as_strided((1, 1, L, 2 * D), (0, 0, apart, 1))
+    rows.copy_(torch.cat([k, v], -1).to(DEV))
+    out = ops.window_attention(q.to(DEV), rows[..., :D], rows[..., D:], 100, 3)
+    see = S.visible([L - T], [T], T, L, 100, 3)
+    attn_check(out, q, k, v, see, dt)

@@ -230,3 +230,12 @@ def test_oracle_rotation_by_complex_turns():
             assert abs(complex(y[0, 0, t, i], y[0, 0, t, i + 3]) - a) < 1e-9
             assert abs(complex(z[0, 0, t, 2 * i], z[0, 0, t, 2 * i + 1]) - b) < 1e-9
         assert torch.equal(y[0, 0, t, 6:], x[0, 0, t, 6:].double())
+
+
+def test_kv_evict_refuses_its_own_table_in_any_type():
+    _, _, pages, table = tensors()
+    w, n = torch.zeros(B, Hk, L), torch.zeros(B, dtype=torch.int64)
+    long = table.long()
+    for t, out in ((long, long), (table, table[:, :6]), (long, long[:, :6])):
+        with pytest.raises(ValueError, match="onto themselves"):
+            ops.kv_evict(w, n, pages, pages, t, out)
