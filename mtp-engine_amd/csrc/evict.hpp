@@ -18,9 +18,12 @@
 // rows move, 16 bytes a lane where the row allows it, the few rows of a small
 // cache by the same workgroup: that part is bound by HBM.
 //
-// Measured (B 4, 8 heads, L 8192, keep 2048, D 128, bf16): selection 12.9 us, move
-// 13.3 us (5.0 TB/s); both as a launch a pass over 8 bits and a thread's entries
-// one by one: selection 31 us.
+// A pass has three barriers, and the passes end where a digit's entries are all
+// wanted, mostly after two.
+//
+// Measured (B 4, 8 heads, L 8192, keep 2048, D 128, bf16): selection 11.6 us, move
+// 13.4 us (5.0 TB/s); with all three passes, five barriers each: selection 12.9 us;
+// a launch a pass over 8 bits and a thread's entries one by one: 31 us.
 #pragma once
 
 #include "mtp_common.hpp"
@@ -71,7 +74,8 @@ __device__ __forceinline__ void evict_copy(const EvictArgs &a, int b, int h, int
 
 constexpr int kEvictThreads = 1024;
 
-// Inclusive sum over the workgroup, and its total; s_sum: one word a wave.
+// Inclusive sum over the workgroup, and its total. s_sum: one word a wave, whose
+// earlier readers have passed a barrier since.
 __device__ __forceinline__ uint32_t evict_scan(uint32_t x, uint32_t *s_sum, uint32_t &total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -79,7 +83,6 @@ __device__ __forceinline__ uint32_t evict_scan(uint32_t x, uint32_t *s_sum, uint
     const uint32_t y = __shfl_up(x, o, 64);
     if (lane >= o) x += y;
   }
-  __syncthreads();  // earlier uses of s_sum
   if (lane == 63) s_sum[wave] = x;
   __syncthreads();
   uint32_t before = 0u;
@@ -99,8 +102,8 @@ template <int E>
 __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const EvictArgs a) {
   constexpr int BINS = 2048;
   constexpr int COPIES = 4;  // of a histogram, lane l in copy l % 4: fewer lanes meet
-  __shared__ uint32_t s_hist[COPIES][BINS + 16];
-  __shared__ uint32_t s_sum[kEvictThreads / 64];
+  __shared__ __attribute__((aligned(8))) uint32_t s_hist[COPIES][BINS + 16];
+  __shared__ uint32_t s_sum[2][kEvictThreads / 64];
   __shared__ uint32_t s_pick[2];
   const int th = threadIdx.x;
   const int bh = blockIdx.x, b = bh / a.Hk, h = bh - b * a.Hk;
@@ -149,16 +152,17 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
 
   // thr, need: the entries to keep are those above thr and the first `need` of
   // its equals. After the pass at bit sh, thr has the bits of the keep-th
-  // largest rank from sh up.
+  // largest rank from sh up; where all that have them are wanted, it is one
+  // less than the least of those, and no pass is left to do.
   uint32_t thr = 0u, need = (uint32_t)a.keep;
+#pragma unroll
+  for (int c = 0; c < COPIES; ++c) s_hist[c][th] = s_hist[c][th + 1024] = 0u;
+  __syncthreads();
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
     const int sh = pass == 0 ? 21 : pass == 1 ? 10 : 0;
     const uint32_t bins = pass == 2 ? 1024u : 2048u;
     const uint32_t mask = pass == 0 ? 0u : ~0u << (pass == 1 ? 21 : 10);
-#pragma unroll
-    for (int c = 0; c < COPIES; ++c) s_hist[c][th] = s_hist[c][th + 1024] = 0u;
-    __syncthreads();
     each_key([&](int, uint32_t u, float) {
       if (u != 0u && (u & mask) == thr) {
         const uint32_t bin = (u >> sh) & (bins - 1u);
@@ -174,15 +178,19 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
       }
     });
     __syncthreads();
-    // from the top: thread th has bins 2047 - 2 th and 2046 - 2 th
+    // from the top: thread th has bins 2047 - 2 th and 2046 - 2 th, and leaves
+    // them clear for the next pass
     uint32_t c0 = 0u, c1 = 0u;
 #pragma unroll
     for (int c = 0; c < COPIES; ++c) {
-      c0 += s_hist[c][BINS - 1 - 2 * th];
-      c1 += s_hist[c][BINS - 2 - 2 * th];
+      uint2 *const two = (uint2 *)&s_hist[c][BINS - 2 - 2 * th];
+      const uint2 x = *two;
+      c0 += x.y;
+      c1 += x.x;
+      *two = uint2{0u, 0u};
     }
     uint32_t total;
-    const uint32_t incl = evict_scan(c0 + c1, s_sum, total);
+    const uint32_t incl = evict_scan(c0 + c1, s_sum[0], total);
     const uint32_t above = incl - c0 - c1;
     if (total < need) {  // fewer entries than wanted (first pass alone): all of them
       thr = 0u;
@@ -191,12 +199,16 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
     }
     if (above < need && incl >= need) {
       const bool hi = above + c0 >= need;
-      s_pick[0] = (uint32_t)(BINS - 1 - 2 * th - (hi ? 0 : 1));
-      s_pick[1] = need - above - (hi ? 0u : c0);
+      const uint32_t low = thr | (uint32_t)(BINS - 1 - 2 * th - (hi ? 0 : 1)) << sh;
+      const uint32_t left = need - above - (hi ? 0u : c0);
+      const bool whole = left == (hi ? c0 : c1);
+      s_pick[0] = whole ? max(low, 1u) - 1u : low;
+      s_pick[1] = whole ? 0u : left;
     }
     __syncthreads();
-    thr |= s_pick[0] << sh;
+    thr = s_pick[0];
     need = s_pick[1];
+    if (need == 0u) break;
   }
 
   uint32_t over = 0u, same = 0u;
@@ -204,10 +216,10 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
     over += u > thr;
     same += (u == thr) & (u != 0u);
   });
-  uint32_t taken, equals;
-  const uint32_t eb = evict_scan(same, s_sum, equals) - same;  // equals before the thread's
+  uint32_t taken, equals, eb = 0u;  // eb: equals before the thread's
+  if (need != 0u) eb = evict_scan(same, s_sum[0], equals) - same;  // after all passes
   const uint32_t mine = over + min(eb + same, need) - min(eb, need);
-  uint32_t at = evict_scan(mine, s_sum, taken) - mine;
+  uint32_t at = evict_scan(mine, s_sum[1], taken) - mine;
   uint32_t es = eb;
   int32_t *const kept = a.kept + (int64_t)bh * a.keep;
   float *const ow = a.out_weights + (int64_t)bh * a.keep;
