@@ -683,8 +683,8 @@ size_t mtp_window_attention_workspace_bytes(int dtype, int64_t B, int64_t H,
  *   out_weights [B, Hk, keep] fp32: their weights, 0 past it
  *   out_lengths [B] int64: entries kept
  * weights [B, Hk, L] fp32, lengths [B] int64, page_table [B, L] int32; pages
- * [num_pages, B, Hk, page_size, row_bytes]; sinks + recent <= keep. Two
- * launches, no workspace.
+ * [num_pages, B, Hk, page_size, row_bytes]; sinks + recent <= keep. One
+ * or two launches, no workspace.
  */
 int mtp_kv_evict(const float *weights, const int64_t *lengths, int64_t B,
                  int64_t Hk, int64_t L, int64_t keep, int64_t sinks,

@@ -19,6 +19,9 @@
 // for all of the token's heads. In the half form the partner element of a
 // pair is the same place of another lane's 16 bytes: the raw row is
 // exchanged (half the lane traffic of fp32 values) and normed on both sides.
+// 4096 tokens of 32 + 8 heads of 128 in bf16 (84 MB): 16.7 us, 5.0 TB/s, what a
+// large copy reaches; 8 tokens: 6.1 us, a launch and the latencies of position,
+// page, rows and store in turn.
 #pragma once
 
 #include "mtp_common.hpp"

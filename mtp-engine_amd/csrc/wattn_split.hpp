@@ -5,9 +5,11 @@
 // The G * T rows of a (sequence, key head) - query heads of a group read the
 // same keys - go by blocks of 16 * RT (row r = t * G + head); a block's
 // visible keys, counted without gaps (WinSpan), are split into nchunks equal
-// parts, one per workgroup, so that few rows still fill the chip; chunks join
-// in win_merge_kernel, in order. Within a workgroup four waves take steps of
-// SK keys in turn and join at the end; a step has no barrier:
+// parts, one per workgroup, so that few rows still fill the chip. The chunks
+// join in their order: by the block's last workgroup to arrive, or in
+// win_join_kernel where there is more to join (or the weights are wanted).
+// Within a workgroup NW waves take steps of SK keys in turn and join at the end;
+// a step has no barrier:
 //   * K and V rows go from memory to registers, whole rows a load, and from
 //     there to the wave's own part of LDS; the next step's rows are asked for
 //     as soon as these have left the registers, their pages one step earlier.
@@ -19,11 +21,15 @@
 //     reads, four keys of one d a lane.
 // The running maximum moves only when a step exceeds it by more than 2^8.
 //
-// Bound: HBM, K and V read once per row block (blocks of one key head run on
-// one XCD and meet in its L2). 16 KB a wave in flight, two waves per SIMD.
-// Loads in the order of the K operand (16 rows of 64 bytes each) instead of
-// whole rows, without LDS for K: 106 us against 92 on 131072 keys of 8 heads
-// (537 MB); three waves per SIMD of smaller chunks: 122.
+// Bound of new tokens: HBM, K and V read once per row block (blocks of one key
+// head run on one XCD and meet in its L2). 16 KB a wave in flight, two waves per
+// SIMD. 131072 keys of 8 heads (537 MB): 87.5 us, 6.1 TB/s; 8 sequences of 1366 ..
+// 4096 keys (101 MB): 23.5 us. The first of these with loads in the order of the
+// K operand (16 rows of 64 bytes each), without LDS for K: 106 us; with three
+// waves per SIMD of smaller chunks: 122. Bound of fp32 prompts: the fp32 matrix
+// instructions, 58 % of their peak (T 4096, 8 heads of 64, no window: 192 us),
+// and the ends of short blocks (B 2, T 1000, window 256, 16 heads: 36 us, where
+// they take 16); blocks of 64 rows: 258 and 40 us.
 #pragma once
 
 #include "wattn_weights.hpp"

