@@ -27,9 +27,10 @@
 // 4096 keys (101 MB): 23.5 us. The first of these with loads in the order of the
 // K operand (16 rows of 64 bytes each), without LDS for K: 106 us; with three
 // waves per SIMD of smaller chunks: 122. Bound of fp32 prompts: the fp32 matrix
-// instructions, 58 % of their peak (T 4096, 8 heads of 64, no window: 192 us),
-// and the ends of short blocks (B 2, T 1000, window 256, 16 heads: 36 us, where
-// they take 16); blocks of 64 rows: 258 and 40 us.
+// instructions and the arithmetic beside them, 65 % of the former's peak (T 4096, 8
+// heads of 64, no window: 173 us; with a shuffle for every row's address instead
+// of scalar arithmetic 192), and the ends of short blocks (B 2, T 1000, window 256,
+// 16 heads: 35 us, where they take 16). Blocks of 64 rows: 258 and 40 us.
 #pragma once
 
 #include "wattn_weights.hpp"
@@ -160,7 +161,23 @@ __global__ void __launch_bounds__(64 * NW, 2) win_split_kernel(const WinArgs a) 
     return (int64_t)((uint64_t)(uint32_t)__shfl((int)(x >> 32), from, 64) << 32 |
                      (uint32_t)__shfl((int)x, from, 64));
   };
+  // dense: the lane's first row and chunk of a step at key 0
+  const char *const kd = (const char *)a.k + (kbase + lane / LPK * a.k_st) * EB + 16 * (lane % LPK);
+  const char *const vd = (const char *)a.v + (vbase + lane / LPK * a.v_st) * EB + 16 * (lane % LPK);
   auto fetch = [&](int st) {
+    if constexpr (!PAGED) {
+      const int i0 = c0 + st * SK;
+      if (i0 >= s.ns && i0 + SK <= c1) {  // whole, keys in a row: addresses by the scalar unit
+        okn = SK == 32 ? 0xffffffffu : 0xffffu;
+        const int64_t j0 = s.lo + (i0 - s.ns);
+#pragma unroll
+        for (int n = 0; n < NL; ++n) {
+          kr[n] = ld16(kd + (j0 + n * KPI) * a.k_st * EB);
+          vr[n] = ld16(vd + (j0 + n * KPI) * a.v_st * EB);
+        }
+        return;
+      }
+    }
     const int i = index_of(st), j = s.key(i);
     bool ok = i < c1;
     int64_t ko, vo;
