@@ -14,16 +14,19 @@
 // 11 and 10 bits a pass from a histogram in LDS (the top 11 are the sign, the
 // exponent and two bits more, so that few lanes meet in one counter), and a
 // prefix sum over the workgroup gives the larger ones and the first of its
-// equals their places. A thread keeps its run of entries in registers. Then the
+// equals their places. A lane keeps its entries in registers. Then the
 // rows move, 16 bytes a lane where the row allows it, the few rows of a small
 // cache by the same workgroup: that part is bound by HBM.
 //
 // A pass has three barriers, and the passes end where a digit's entries are all
 // wanted, mostly after two.
 //
-// Measured (B 4, 8 heads, L 8192, keep 2048, D 128, bf16): selection 11.6 us, move
+// Measured (B 4, 8 heads, L 8192, keep 2048, D 128, bf16): selection 11.3 us, move
 // 13.4 us (5.0 TB/s); with all three passes, five barriers each: selection 12.9 us;
-// a launch a pass over 8 bits and a thread's entries one by one: 31 us.
+// a launch a pass over 8 bits and a thread's entries one by one: 31 us. 16 heads of
+// 31391 entries, keep 5042, D 64: 34.4 us both, with a thread's entries one after
+// another in memory 59; 16 heads of 100000 entries, keep 4096, D 128: 120 and 525,
+// the arithmetic of one CU a head.
 #pragma once
 
 #include "mtp_common.hpp"
@@ -38,7 +41,6 @@ struct EvictArgs {
   int B, Hk, L, keep, sinks, recent, npages, page_size;
   void *k_pages, *v_pages;     // [P, B, Hk, page_size, D], by bytes: from and to
   int64_t row_bytes;
-  int quads;                   // weights and tables in whole 16 bytes a row
   int moves;                   // 1: the selecting workgroup moves its rows (16-byte units)
   int32_t *kept;               // [B, Hk, keep], -1 past the new length
   float *out_weights;          // [B, Hk, keep], 0 past it
@@ -96,57 +98,76 @@ __device__ __forceinline__ uint32_t evict_scan(uint32_t x, uint32_t *s_sum, uint
   return x + before;
 }
 
-// E: entries of a thread in registers, thread th the entries th * E .. + E - 1
-// (E * kEvictThreads >= L); 0: any number, read again for every pass.
+// E: entries of a lane in registers (E * kEvictThreads >= L); 0: any number, read
+// again for every pass. A wave has `each` runs of 256 entries one after another, a
+// lane four in a row of each run, so that loads are whole lines and ballots give
+// the places within a run.
 template <int E>
 __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const EvictArgs a) {
   constexpr int BINS = 2048;
   constexpr int COPIES = 4;  // of a histogram, lane l in copy l % 4: fewer lanes meet
+  constexpr int WAVES = kEvictThreads / 64;
   __shared__ __attribute__((aligned(8))) uint32_t s_hist[COPIES][BINS + 16];
-  __shared__ uint32_t s_sum[2][kEvictThreads / 64];
+  __shared__ uint32_t s_sum[WAVES];
+  __shared__ uint2 s_cnt[WAVES];
   __shared__ uint32_t s_pick[2];
-  const int th = threadIdx.x;
+  const int th = threadIdx.x, lane = th & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(th >> 6);
   const int bh = blockIdx.x, b = bh / a.Hk, h = bh - b * a.Hk;
   const float *const w = a.weights + (int64_t)bh * a.L;
   const int32_t *const tab = a.table + (int64_t)b * a.L;
   const int n = (int)min(max(a.lengths[b], (int64_t)0), (int64_t)a.L);
-  const int each = E ? E : (n + kEvictThreads - 1) / kEvictThreads;
-  const int j0 = min((int64_t)th * each, (int64_t)n);  // the thread's entries: j0 .. j1 - 1
-  const int j1 = min((int64_t)j0 + each, (int64_t)n);
-
-  uint32_t key[E ? E : 1];
-  float val[E ? E : 1];
-  if constexpr (E > 0) {
-    // every load before the first use (n - 1 in place of entries past the end)
-    int pg[E];
-    if (a.quads && th * E + E <= n) {  // rows of whole 16 bytes
+  const int each = (n + 4 * kEvictThreads - 1) / (4 * kEvictThreads);
+  const int j0 = (wave * each * 64 + lane) * 4;  // below n + 2^13
+  auto load4 = [&](int j, float (&x)[4], int (&pg)[4]) {
+    if (j + 4 <= n) {  // 16 bytes, of any row at a word's alignment
+      typedef __attribute__((ext_vector_type(4), aligned(4))) float f32x4w;
+      typedef __attribute__((ext_vector_type(4), aligned(4))) uint32_t u32x4w;
+      const f32x4w x4 = *(const f32x4w *)(w + j);
+      const u32x4w p4 = *(const u32x4w *)(tab + j);
 #pragma unroll
-      for (int e = 0; e < E; e += 4) {
-        const f32x4 x4 = *(const f32x4 *)(w + th * E + e);
-        const u32x4 p4 = *(const u32x4 *)(tab + th * E + e);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          val[e + i] = x4[i];
-          pg[e + i] = (int)p4[i];
-        }
+      for (int i = 0; i < 4; ++i) {
+        x[i] = x4[i];
+        pg[i] = (int)p4[i];
       }
-    } else {
+    } else {  // the last one in place of entries past the end
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int j = min(th * E + e, max(n - 1, 0));
-        val[e] = n > 0 ? w[j] : 0.f;
-        pg[e] = n > 0 ? tab[j] : -1;
+      for (int i = 0; i < 4; ++i) {
+        x[i] = w[min(j + i, n - 1)];
+        pg[i] = tab[min(j + i, n - 1)];
       }
     }
+  };
+
+  constexpr int Q = E ? E / 4 : 1;
+  uint32_t key[Q][4];
+  float val[Q][4];
+  if constexpr (E > 0) {
+    int pg[Q][4];  // every load before the first use
 #pragma unroll
-    for (int e = 0; e < E; ++e) key[e] = evict_key(a, n, th * E + e, val[e], pg[e]);
+    for (int q = 0; q < Q; ++q)
+      if (q < each) load4(j0 + 256 * q, val[q], pg[q]);
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        key[q][i] = q < each ? evict_key(a, n, j0 + 256 * q + i, val[q][i], pg[q][i]) : 0u;
   }
-  auto each_key = [&](auto f) {  // f(entry, rank, weight) over the thread's entries
+  // f(first entry, ranks, weights) over the wave's runs, all its lanes together
+  auto each_quad = [&](auto f) {
     if constexpr (E > 0) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) f(th * E + e, key[e], val[e]);
+      for (int q = 0; q < Q; ++q)
+        if (q < each) f(j0 + 256 * q, key[q], val[q]);
     } else {
-      for (int j = j0; j < j1; ++j) f(j, evict_key(a, n, j, w[j], tab[j]), w[j]);
+      for (int q = 0; q < each; ++q) {
+        const int j = j0 + 256 * q;
+        int pg[4];
+        load4(j, val[0], pg);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) key[0][i] = evict_key(a, n, j + i, val[0][i], pg[i]);
+        f(j, key[0], val[0]);
+      }
     }
   };
 
@@ -163,17 +184,21 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
     const int sh = pass == 0 ? 21 : pass == 1 ? 10 : 0;
     const uint32_t bins = pass == 2 ? 1024u : 2048u;
     const uint32_t mask = pass == 0 ? 0u : ~0u << (pass == 1 ? 21 : 10);
-    each_key([&](int, uint32_t u, float) {
-      if (u != 0u && (u & mask) == thr) {
-        const uint32_t bin = (u >> sh) & (bins - 1u);
-        // lanes of one bin add once (equal weights, above all zeros)
-        const uint32_t first = (uint32_t)__builtin_amdgcn_readfirstlane((int)bin);
-        const unsigned long long all = __ballot(1);
-        if (__ballot(bin == first) == all) {
-          if ((int)(threadIdx.x & 63) == __builtin_ctzll(all))
-            atomicAdd(&s_hist[0][bin], (uint32_t)__popcll(all));
-        } else {
-          atomicAdd(&s_hist[th % COPIES][bin], 1u);
+    each_quad([&](int, const uint32_t(&k)[4], const float(&)[4]) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t u = k[i];
+        if (u != 0u && (u & mask) == thr) {
+          const uint32_t bin = (u >> sh) & (bins - 1u);
+          // lanes of one bin add once (equal weights, above all zeros)
+          const uint32_t first = (uint32_t)__builtin_amdgcn_readfirstlane((int)bin);
+          const unsigned long long all = __ballot(1);
+          if (__ballot(bin == first) == all) {
+            if (lane == __builtin_ctzll(all))
+              atomicAdd(&s_hist[0][bin], (uint32_t)__popcll(all));
+          } else {
+            atomicAdd(&s_hist[lane % COPIES][bin], 1u);
+          }
         }
       }
     });
@@ -190,7 +215,7 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
       *two = uint2{0u, 0u};
     }
     uint32_t total;
-    const uint32_t incl = evict_scan(c0 + c1, s_sum[0], total);
+    const uint32_t incl = evict_scan(c0 + c1, s_sum, total);
     const uint32_t above = incl - c0 - c1;
     if (total < need) {  // fewer entries than wanted (first pass alone): all of them
       thr = 0u;
@@ -211,28 +236,71 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
     if (need == 0u) break;
   }
 
+  // places: entries above thr and equals of it in the waves before
   uint32_t over = 0u, same = 0u;
-  each_key([&](int, uint32_t u, float) {
-    over += u > thr;
-    same += (u == thr) & (u != 0u);
+  each_quad([&](int, const uint32_t(&k)[4], const float(&)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      over += (uint32_t)__popcll(__ballot(k[i] > thr));
+      if (need != 0u) same += (uint32_t)__popcll(__ballot((k[i] == thr) & (k[i] != 0u)));
+    }
   });
-  uint32_t taken, equals, eb = 0u;  // eb: equals before the thread's
-  if (need != 0u) eb = evict_scan(same, s_sum[0], equals) - same;  // after all passes
-  const uint32_t mine = over + min(eb + same, need) - min(eb, need);
-  uint32_t at = evict_scan(mine, s_sum[1], taken) - mine;
-  uint32_t es = eb;
+  if (lane == 0) s_cnt[wave] = uint2{over, same};
+  __syncthreads();
+  uint32_t at = 0u, es = 0u, all = 0u, equals = 0u;
+#pragma unroll
+  for (int x = 0; x < WAVES; ++x) {
+    const uint2 c = s_cnt[x];
+    at += x < wave ? c.x : 0u;
+    es += x < wave ? c.y : 0u;
+    all += c.x;
+    equals += c.y;
+  }
+  const uint32_t taken = all + min(equals, need);
+  at += min(es, need);
   int32_t *const kept = a.kept + (int64_t)bh * a.keep;
   float *const ow = a.out_weights + (int64_t)bh * a.keep;
-  each_key([&](int j, uint32_t u, float x) {
-    const bool eq = (u == thr) & (u != 0u);
-    if (u > thr || (eq && es < need)) {
-      if (at < (uint32_t)a.keep) {
-        kept[at] = j;
-        ow[at] = x;
+  auto before = [&](unsigned long long m, uint32_t x) {  // x and the lanes below in m
+    return (uint32_t)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32),
+                                               __builtin_amdgcn_mbcnt_lo((uint32_t)m, x));
+  };
+  each_quad([&](int j, const uint32_t(&k)[4], const float(&x)[4]) {
+    // those taken in the lanes before, then in this lane
+    bool take[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) take[i] = k[i] > thr;
+    if (need != 0u) {  // equals too, by their rank
+      uint32_t rank = es;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const unsigned long long m = __ballot((k[i] == thr) & (k[i] != 0u));
+        rank = before(m, rank);
+        es += (uint32_t)__popcll(m);
       }
-      ++at;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool eq = (k[i] == thr) & (k[i] != 0u);
+        take[i] = take[i] | (eq & (rank < need));
+        rank += eq;
+      }
     }
-    es += eq;
+    uint32_t to = at;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const unsigned long long m = __ballot(take[i]);
+      to = before(m, to);
+      at += (uint32_t)__popcll(m);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (take[i]) {
+        if (to < (uint32_t)a.keep) {
+          kept[to] = j + i;
+          ow[to] = x[i];
+        }
+        ++to;
+      }
+    }
   });
   for (int j = (int)taken + th; j < a.keep; j += kEvictThreads) {
     kept[j] = -1;

@@ -459,8 +459,7 @@ int mtp_kv_evict(const float *weights, const int64_t *lengths, int64_t B, int64_
   // (against a second launch: 64 KB of 8 heads 14.4 us and 15.9, 128 KB of 8
   // 16.7 and 16.5, of 64 heads 21.9 and 17.1)
   a.moves = num_pages > 0 && unit == 16 && keep * row_bytes <= 64 << 10;
-  a.quads = L % 4 == 0 && aligned16(weights) && aligned16(page_table);
-  // entries of a thread kept in registers, where they fit
+  // entries of a lane kept in registers, where they fit
   const int64_t each = (L + kEvictThreads - 1) / kEvictThreads;
   void (*const sel)(EvictArgs) = each <= 4    ? evict_select_kernel<4>
                                  : each <= 8  ? evict_select_kernel<8>

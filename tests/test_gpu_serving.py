@@ -770,3 +770,22 @@ def test_dense_keys_past_32_bits(dt):
     out = ops.window_attention(q.to(DEV), rows[..., :D], rows[..., D:], 100, 3)
     see = S.visible([L - T], [T], T, L, 100, 3)
     attn_check(out, q, k, v, see, dt)
+
+
+@pytest.mark.parametrize("L,n,keep", [(1000, 997, 300), (5003, 5003, 2000), (40003, 40001, 700)])
+def test_kv_evict_ties_across_lanes(L, n, keep):
+    """Few distinct weights, so that the last ones kept are equals of many that are
+    not, in lanes and waves on both sides; rows that start at any word."""
+    from mtp_hip import ops
+    g = gen(L)
+    B, Hk, page = 1, 3, 16
+    P = L // page + keep // page + 4
+    w = torch.randint(0, 4, (B, Hk, L), generator=g).float()
+    kp, vp, table, out_table = make_pages(g, P, B, Hk, page, 4, L, BF16, keep)
+    kept, ow, new = ops.kv_evict(w.to(DEV), torch.tensor([n]).to(DEV), kp.to(DEV), vp.to(DEV),
+                                 table.to(DEV), out_table.to(DEV), 3, 50)
+    key = w[..., :n].double()
+    key[..., :3] = key[..., n - 50:] = math.inf
+    ref = torch.sort(key, dim=-1, descending=True, stable=True).indices[..., :keep].sort(-1).values
+    assert torch.equal(kept.cpu().long(), ref) and int(new) == keep
+    assert torch.equal(ow.cpu(), torch.gather(w, 2, ref))
