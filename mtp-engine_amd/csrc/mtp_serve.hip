@@ -126,7 +126,7 @@ int rope_args(RopeArgs &a, const mtp_rope_args *p) {
 
 // ---- windowed attention
 struct WinPlan {
-  bool prompt = false;     // the prompt kernel, where the strides let it
+  int prompt = 0;          // chunks of the prompt kernel, where the strides let it take the call
   int rt = 0;              // else the split kernel: row tiles of a block; 0: one wave per row
   int nw = 4;              // its waves
   int rblocks = 1, nchunks = 1;
@@ -145,28 +145,38 @@ int win_window(int64_t window) {
   return window < 0 || window >= kWinNone / 2 ? kWinNone : (int)window;
 }
 
-// Whether dense 16-bit rows take the prompt kernel: the estimates of both
-// kernels' times, in us, fitted to 176 sizes (head dim 64 and 128; 1 .. 32
-// (batch, key head) pairs, 33 .. 17500 rows, 33 .. 4000 keys, no window):
+// Chunks of keys with which dense 16-bit rows take the prompt kernel; 0: the split
+// kernel. By estimates of the times, in us, fitted to 176 sizes (head dim 64 and
+// 128; 1 .. 32 (batch, key head) pairs, 33 .. 17500 rows, 33 .. 4000 keys, no
+// window):
 //   prompt  5 + 1.25 a tile of the longest block, or 1.6 a tile over the 512
-//           blocks that run at once (head dim 64: 4, 0.9 and 1.1)
+//           blocks that run at once (head dim 64: 4, 0.9 and 1.1); with chunks 6
+//           more and the partials' bytes at 3 TB/s
 //   split   8 + 45 a million keys of all the 32-row blocks (head dim 64: 7, 28)
 // e.g. at head dim 128: 32 pairs, T 1000, L 1000: 27.9 and 38.7 us measured; 8
-// pairs, T 1000, L 4000: 85.0 and 50.8; one pair of 33 rows and keys: 5.6, 8.1.
-bool win_takes_prompt(int dt, int64_t units, int64_t G, int64_t T, int64_t D, int64_t L,
+// pairs, T 1000, L 4000: 85.0 and 50.8; one pair of 33 rows and keys: 5.6, 8.1. 8
+// pairs of four heads, T 512: L 8192 92.6 with chunks, 170 with one or split; L
+// 32768 307 and 733.
+int win_prompt_chunks(int dt, int64_t units, int64_t G, int64_t T, int64_t D, int64_t L,
                       int64_t window, int64_t sinks) {
-  if (!win_prompt_pick(dt, (int)std::min<int64_t>(D, 1 << 20))) return false;
+  if (!win_prompt_pick(dt, (int)std::min<int64_t>(D, 1 << 20))) return 0;
   const double rows = (double)(G * T);
-  const double mean = (double)std::min(win_most(1, L, window, sinks), std::max<int64_t>(1, L - T / 2));
+  const double mean =
+      (double)std::min(win_most(1, L, window, sinks), std::max<int64_t>(1, L - T / 2));
   const double most = (double)win_most(std::min(T, kWinPromptRows / G + 2), L, window, sinks);
   const double blocks = std::ceil(rows / kWinPromptRows) * units;
   const bool small = D == 64;
-  const double prompt = (small ? 4. : 5.) +
-                        std::max((small ? 0.9 : 1.25) * std::ceil(most / kWinTileKeys),
-                                 (small ? 1.1 : 1.6) * blocks * (mean / kWinTileKeys + 1.) / 512.);
-  const double split = (small ? 7. : 8.) +
-                       (small ? 28e-6 : 45e-6) * std::ceil(rows / 32.) * units * (mean + 32.);
-  return prompt < split;
+  double best = (small ? 7. : 8.) +
+                (small ? 28e-6 : 45e-6) * std::ceil(rows / 32.) * units * (mean + 32.);
+  int chunks = 0;
+  for (int c = 1; c <= 8 && (c == 1 || blocks * c <= 512.); c *= 2) {
+    const double t = (small ? 4. : 5.) +
+                     std::max((small ? 0.9 : 1.25) * std::ceil(most / kWinTileKeys / c),
+                              (small ? 1.1 : 1.6) * blocks * (mean / kWinTileKeys + c) / 512.) +
+                     (c > 1 ? 6. + 8e-6 / 3. * rows * units * c * D : 0.);
+    if (t < best) best = t, chunks = c;
+  }
+  return chunks;
 }
 
 // Rows of 16 whole bytes at 64 or 128 elements take the split kernel, dense
@@ -178,7 +188,7 @@ WinPlan win_plan(int dt, int64_t B, int64_t H, int64_t Hk, int64_t T, int64_t D,
   const int64_t rows = H / Hk * T, units = B * Hk;
   size_t at = kCounterBytes;
   if (win_split_pick(dt, (int)std::min<int64_t>(D, 1 << 20), 1, false, 4)) {
-    p.prompt = !paged && win_takes_prompt(dt, units, H / Hk, T, D, L, window, sinks);
+    p.prompt = paged ? 0 : win_prompt_chunks(dt, units, H / Hk, T, D, L, window, sinks);
     p.rt = rows > 16 ? 2 : 1;
     const int64_t rp = 16 * p.rt;
     p.rblocks = (int)((rows + rp - 1) / rp);
@@ -195,12 +205,15 @@ WinPlan win_plan(int dt, int64_t B, int64_t H, int64_t Hk, int64_t T, int64_t D,
     // 32 KB: 15.0 and 15.6; 128 KB: 12.2 and 13.8; 256 KB: 16.7 and 14.8)
     p.joined = p.nchunks > 1 && !weights && p.nchunks <= kWinTicketChunks &&
                std::min(rp, rows) * p.nchunks * D * 4 <= 128 << 10 && wgs <= kCounterSlots;
-    const int64_t parts = wgs * p.nchunks * rp;
-    if (p.nchunks > 1) {
+    const int64_t pblocks = (rows + kWinPromptRows - 1) / kWinPromptRows;
+    const int64_t parts =
+        p.prompt > 1 ? units * pblocks * p.prompt * kWinPromptRows : wgs * p.nchunks * rp;
+    const bool chunks = p.prompt > 1 || p.nchunks > 1;
+    if (chunks) {
       p.part_off = at;
       at += align_up((size_t)parts * (size_t)D * 4, 256);
     }
-    if (p.nchunks > 1 || weights) {
+    if (chunks || weights) {
       p.pml_off = at;
       at += align_up((size_t)std::max(parts, B * H * T) * 8, 256);
     }
@@ -257,34 +270,39 @@ int win_launch(WinArgs &a, int dt, void *workspace, size_t workspace_bytes, hipS
                     (a.L - 1) * a.v_st < reach;
   const int64_t pblocks = ((int64_t)a.G * a.T + kWinPromptRows - 1) / kWinPromptRows;
   // (its maximum is that of the products, so it takes no scale below zero)
+  // the chunks' join, and the weights
+  const bool paged = a.table != nullptr;
+  auto join = [&]() {
+    // four waves to a row of many chunks while the chip has room for them
+    const int mw = a.nchunks > 8 && rows <= 8 * (int64_t)device_cus() ? 4 : 1;
+    a.joins = a.nchunks > 1 ? (int)((rows * mw + 3) / 4) : 0;
+    const int64_t sums = a.weights ? (p.ld_sc + 255) / 256 * a.B * a.Hk : 0;
+    if (a.joins + sums > INT32_MAX) return (int)MTP_ERR_SHAPE;
+    hipLaunchKernelGGL(win_join_pick(dt, a.D, paged, mw), dim3((unsigned)(a.joins + sums)),
+                       dim3(256), 0, st, a);
+    return launch_status();
+  };
   if (p.prompt && near && whole && a.scale > 0.f && pblocks <= 65535) {
     a.rblocks = (int)pblocks;
-    hipLaunchKernelGGL(win_prompt_pick(dt, a.D), dim3((unsigned)(a.B * a.Hk), (unsigned)pblocks),
-                       dim3(kWinPromptRows * 2),
-                       win_prompt_lds(a.D), st, a);
-    return launch_status();
+    a.rp = kWinPromptRows;
+    a.nchunks = p.prompt;
+    hipLaunchKernelGGL(
+        win_prompt_pick(dt, a.D),
+        dim3((unsigned)(a.B * a.Hk), (unsigned)pblocks, (unsigned)p.prompt),
+        dim3(kWinPromptRows * 2), win_prompt_lds(a.D), st, a);
+    s = launch_status();
+    return s == MTP_OK && p.prompt > 1 ? join() : s;
   }
   if (p.rt && whole && p.rblocks <= 65535) {
     a.rblocks = p.rblocks;
     a.rp = 16 * p.rt;
     a.nchunks = p.nchunks;
     a.ticket = p.joined ? (unsigned *)w8 : nullptr;
-    const bool paged = a.table != nullptr;
     hipLaunchKernelGGL(win_split_pick(dt, a.D, p.rt, paged, p.nw),
                        dim3((unsigned)(a.B * a.Hk), (unsigned)p.rblocks, (unsigned)p.nchunks),
                        dim3(64 * p.nw), 0, st, a);
     s = launch_status();
-    if (s == MTP_OK && !p.joined && (p.nchunks > 1 || a.weights)) {
-      // four waves to a row of many chunks while the chip has room for them
-      const int mw = p.nchunks > 8 && rows <= 8 * (int64_t)device_cus() ? 4 : 1;
-      a.joins = p.nchunks > 1 ? (int)((rows * mw + 3) / 4) : 0;
-      const int64_t sums = a.weights ? (p.ld_sc + 255) / 256 * a.B * a.Hk : 0;
-      if (a.joins + sums > INT32_MAX) return MTP_ERR_SHAPE;
-      hipLaunchKernelGGL(win_join_pick(dt, a.D, paged, mw), dim3((unsigned)(a.joins + sums)),
-                         dim3(256), 0, st, a);
-      s = launch_status();
-    }
-    return s;
+    return s == MTP_OK && !p.joined && (p.nchunks > 1 || a.weights) ? join() : s;
   }
   a.rblocks = 1;
   a.rp = a.G * a.T;

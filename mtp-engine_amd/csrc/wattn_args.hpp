@@ -74,7 +74,7 @@ WinKernel win_join_pick(int ct, int d, bool paged, int waves);
 
 // The prompt kernel (wattn_prompt.hpp) for 16-bit rows of head dim d: blocks of
 // kWinPromptRows rows, two threads each, tiles of kWinTileKeys keys; null for
-// other shapes. Grid (B * Hk, row blocks).
+// other shapes. Grid (B * Hk, row blocks, chunks).
 constexpr int kWinPromptRows = 128, kWinTileKeys = 64;
 WinKernel win_prompt_pick(int ct, int d);
 constexpr int win_prompt_lds(int d) { return 2 * 2 * kWinTileKeys * 2 * d; }

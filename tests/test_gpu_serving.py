@@ -789,3 +789,58 @@ def test_kv_evict_ties_across_lanes(L, n, keep):
     ref = torch.sort(key, dim=-1, descending=True, stable=True).indices[..., :keep].sort(-1).values
     assert torch.equal(kept.cpu().long(), ref) and int(new) == keep
     assert torch.equal(ow.cpu(), torch.gather(w, 2, ref))
+
+
+@pytest.mark.parametrize("dt,n,T,L,H,Hk,D,window,sinks", [
+    (F16, [7000], 500, 7000, 16, 8, 64, None, 0), (BF16, [8000], 260, 8000, 8, 4, 128, None, 0),
+    (BF16, [8000, 7601, 5, 7900], 400, 8000, 4, 2, 128, None, 0),
+    (F16, [9000, 8999, 0, 8800], 300, 9000, 8, 4, 64, 8500, 40)])
+def test_chunk_behind_many_keys(dt, n, T, L, H, Hk, D, window, sinks):
+    """Some hundred rows behind thousands of keys (few blocks, their keys in chunks),
+    ragged with garbage behind, and a value that only some rows see."""
+    from mtp_hip import ops
+    g = gen(T + L)
+    B = len(n)
+    print(f"case chunk {dt} {(n, T, L, H, Hk, D, window, sinks)}", flush=True)
+    q, k, v = (randn(g, B, h, m, D, dtype=dt) for h, m in ((H, T), (Hk, L), (Hk, L)))
+    for b in range(B):
+        k[b, :, n[b]:] = math.nan
+        v[b, :, n[b]:] = math.inf
+        q[b, :, max(0, n[b] - (L - T)):] = math.nan
+    dev = [x.to(DEV) for x in (q, k, v)]
+    lengths = torch.tensor(n).to(DEV) if B > 1 else None
+    out = ops.window_attention(*dev, window, sinks, lengths=lengths)
+    see = S.visible([L - T] * B, [max(0, e - (L - T)) for e in n], T, L, window, sinks)
+    attn_check(out, q.nan_to_num(), k.nan_to_num(), v.nan_to_num(posinf=0.0), see, dt)
+    assert torch.equal(out, ops.window_attention(*dev, window, sinks, lengths=lengths))
+    dev[2][0, :, L - T + 10, 2] = math.nan
+    bad = ops.window_attention(*dev, window, sinks, lengths=lengths)
+    assert torch.isnan(bad[0, :, 10:, 2]).all()
+    assert torch.equal(bad[0, :, :10], out[0, :, :10]) or \
+        torch.isfinite(bad[0, :, :10]).all()
+    assert torch.equal(bad[1:], out[1:])
+
+
+def test_chunks_captured_and_replayed():
+    """Keys in chunks and their join as a graph, replayed among eager calls."""
+    from mtp_hip import ops
+    g = gen(31)
+    q, k, v = (randn(g, 1, h, m, 64, dtype=BF16).to(DEV) for h, m in ((8, 300), (4, 9000), (4, 9000)))
+    want = [ops.window_attention(q * s, k, v).clone() for s in (1, 2, 3)]
+    x = q.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.window_attention(x, k, v)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = ops.window_attention(x, k, v)
+    for s in (1, 2, 3):
+        x.copy_(q * s)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[s - 1])
+        ops.window_attention(q, k, v)
+        torch.cuda.synchronize()
