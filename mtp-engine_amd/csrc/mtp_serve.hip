@@ -436,7 +436,8 @@ int mtp_paged_window_attention(const mtp_window_args *p, void *stream) {
 
 int mtp_kv_evict(const float *weights, const int64_t *lengths, int64_t B, int64_t Hk, int64_t L,
                  int64_t keep, int64_t sinks, int64_t recent, void *k_pages, void *v_pages,
-                 int64_t num_pages, int64_t page_size, int64_t row_bytes, const int32_t *page_table, const int32_t *out_table,
+                 int64_t num_pages, int64_t page_size, int64_t row_bytes,
+                 const int32_t *page_table, const int32_t *out_table,
                  int32_t *kept, float *out_weights, int64_t *out_lengths, void *stream) {
   if (B < 0 || Hk < 0 || L < 0 || keep <= 0 || row_bytes <= 0 || num_pages < 0 ||
       page_size <= 0 || num_pages > INT32_MAX || page_size > INT32_MAX || L > kWinMaxKeys ||

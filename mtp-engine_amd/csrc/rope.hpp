@@ -260,7 +260,8 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeArgs a) {
       } else if (st < steps) {
         const int r = (st - nq - nk) * RPI + sub;
         if (on && r < a.Hk && slot >= 0)
-          *(u32x4 *)((char *)a.v_pages + (slot + (int64_t)r * a.p_sh + d0) * dtype_bytes(DT)) = x[u];
+          *(u32x4 *)((char *)a.v_pages + (slot + (int64_t)r * a.p_sh + d0) * dtype_bytes(DT)) =
+              x[u];
       }
     }
   }

@@ -103,7 +103,8 @@ __global__ void __launch_bounds__(64 * NW, 2) win_split_kernel(const WinArgs a) 
   const WinSpan s = win_span(a, b, row0 / a.G, (min(nrows, row0 + RP) - 1) / a.G + 1);
   const int n = s.count();
   const int per = win_chunk<SK>(n, a.nchunks);
-  const int c0 = (int)min((int64_t)n, (int64_t)c * per), c1 = (int)min((int64_t)n, (int64_t)c0 + per);
+  const int c0 = (int)min((int64_t)n, (int64_t)c * per);
+  const int c1 = (int)min((int64_t)n, (int64_t)c0 + per);
   const int64_t unit = (((int64_t)bh * a.rblocks + rb) * a.nchunks + c) * RP;  // its rows' partials
   if (c0 >= c1 && a.nchunks > 1 && !a.ticket) {  // a chunk without keys
     if (th < RP) {
